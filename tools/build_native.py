@@ -40,7 +40,9 @@ def sources() -> list[Path]:
 
 
 def headers_mtime() -> float:
-    return max((p.stat().st_mtime for p in (CSRC / "include").rglob("*.hpp")), default=0.0)
+    """Newest header, or this file (its flags): objects older than that are rebuilt."""
+    deps = list((CSRC / "include").rglob("*.hpp")) + [Path(__file__)]
+    return max(p.stat().st_mtime for p in deps)
 
 
 def compile_one(src: Path, obj: Path, flags: list[str], hdr_mtime: float) -> tuple[Path, str]:
@@ -72,6 +74,10 @@ def build(debug: bool = False, jobs: int | None = None, verbose: bool = False) -
         "-Wno-unused-variable",
         "-Wno-unused-function",
         "-Wno-sign-compare",
+        # no packed-f32 instructions (v_pk_add / mul / fma_f32) in device code:
+        # some of their forms have given wrong results on gfx950. The host pass
+        # does not know the feature and says so.
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-fvisibility=hidden",
         f"-I{CSRC / 'include'}",
         f"-I{py_inc}",
