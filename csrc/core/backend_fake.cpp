@@ -446,6 +446,22 @@ class FakeBackend : public Backend {
     run(s, [a] { attn_decode_cpu(a); });
     return Status::OK;
   }
+  Status paged_plan(int, const PlanArgs& a, void* s) override {
+    run(s, [a] { paged_plan_cpu(a); });
+    return Status::OK;
+  }
+  Status paged_rope(int, const PagedRopeArgs& a, void* s) override {
+    run(s, [a] { paged_rope_cpu(a); });
+    return Status::OK;
+  }
+  Status paged_attn(int, const PagedAttnArgs& a, void* s) override {
+    run(s, [a] { paged_attn_cpu(a); });
+    return Status::OK;
+  }
+  Status verify_draft(int, const VerifyArgs& a, void* s) override {
+    run(s, [a] { verify_draft_cpu(a); });
+    return Status::OK;
+  }
   Status gather_pages(int, const PageListDesc& d, void* s) override {
     std::vector<uint32_t> idx(d.idx, d.idx + d.npages);
     PageListDesc dd = d;

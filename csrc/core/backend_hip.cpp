@@ -62,6 +62,19 @@ namespace {
     }                                                                                  \
   } while (0)
 
+// Makes `dev` the calling thread's current device for a launch on one of its
+// streams, and the earlier one current again.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(int dev) {
+    int cur = -1;
+    if (hipGetDevice(&cur) == hipSuccess && cur != dev && hipSetDevice(dev) == hipSuccess) before = cur;
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
 class HipBackend : public Backend {
  public:
   explicit HipBackend(int n) : ndev_(n) {}
@@ -799,6 +812,26 @@ class HipBackend : public Backend {
   }
   Status attn_decode(int, const AttnArgs& a, void* s) override {
     HIPCHK(launch_attn_decode(a, (hipStream_t)s));
+    return Status::OK;
+  }
+  Status paged_plan(int dev, const PlanArgs& a, void* s) override {
+    DeviceScope on(dev);
+    HIPCHK(launch_paged_plan(a, (hipStream_t)s));
+    return Status::OK;
+  }
+  Status paged_rope(int dev, const PagedRopeArgs& a, void* s) override {
+    DeviceScope on(dev);
+    HIPCHK(launch_paged_rope(a, (hipStream_t)s));
+    return Status::OK;
+  }
+  Status paged_attn(int dev, const PagedAttnArgs& a, void* s) override {
+    DeviceScope on(dev);
+    HIPCHK(launch_paged_attn(a, (hipStream_t)s));
+    return Status::OK;
+  }
+  Status verify_draft(int dev, const VerifyArgs& a, void* s) override {
+    DeviceScope on(dev);
+    HIPCHK(launch_verify_draft(a, (hipStream_t)s));
     return Status::OK;
   }
 

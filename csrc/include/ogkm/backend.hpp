@@ -19,6 +19,7 @@
 
 #include "ogkm/common.hpp"
 #include "ogkm/dgemm.hpp"
+#include "ogkm/paged.hpp"
 
 namespace ogkm {
 
@@ -194,6 +195,11 @@ class Backend {
   virtual Status rmsnorm(int dev, const ResidNormArgs& a, void* stream) = 0;
   virtual Status rope_kv(int dev, const RopeKvArgs& a, void* stream) = 0;
   virtual Status attn_decode(int dev, const AttnArgs& a, void* stream) = 0;
+  // Serving over a paged KV cache, speculative decoding (ogkm/paged.hpp).
+  virtual Status paged_plan(int dev, const PlanArgs& a, void* stream) = 0;
+  virtual Status paged_rope(int dev, const PagedRopeArgs& a, void* stream) = 0;
+  virtual Status paged_attn(int dev, const PagedAttnArgs& a, void* stream) = 0;
+  virtual Status verify_draft(int dev, const VerifyArgs& a, void* stream) = 0;
   virtual Status gather_pages(int dev, const PageListDesc& d, void* stream) = 0;
   virtual Status scatter_pages(int dev, const PageListDesc& d, void* stream) = 0;
   // Asynchronous error state of a stream after its work completed (a kernel or

@@ -15,6 +15,7 @@
 
 #include "ogkm/dgemm.hpp"
 #include "ogkm/fault_abi.hpp"
+#include "ogkm/paged.hpp"
 
 namespace ogkm {
 
@@ -105,6 +106,12 @@ hipError_t launch_dgemm_reduce(const DGemmReduceArgs& a, hipStream_t s);
 hipError_t launch_rmsnorm(const ResidNormArgs& a, hipStream_t s);
 hipError_t launch_rope_kv(const RopeKvArgs& a, hipStream_t s);
 hipError_t launch_attn_decode(AttnArgs a, hipStream_t s);
+// Paged serving (csrc/kernels/paged_ops.hip, paged_attn.hip, speculative.hip);
+// argument structs in ogkm/paged.hpp.
+hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t s);
+hipError_t launch_paged_rope(const PagedRopeArgs& a, hipStream_t s);
+hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t s);
+hipError_t launch_verify_draft(const VerifyArgs& a, hipStream_t s);
 
 // Device fault buffer (GET/PUT ring, ogkm/fault_abi.hpp) as kernels see it.
 struct KFaultBuf {
