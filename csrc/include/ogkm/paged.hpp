@@ -50,6 +50,20 @@ struct PagedRopeArgs {
   uint32_t elem;             // ELEM_BF16 / ELEM_F16
 };
 
+// How a call's work is laid out: from the host's bounds alone, so that one layout
+// serves every content of the device's lengths.
+struct PagedAttnPlan {
+  uint32_t few_rows;    // requests of up to so many rows per kv head take the `few` body
+  uint32_t few_blocks;  // its column blocks of 16 rows: 1, 2 or 4
+  uint32_t few_splits;  // its splits of the key axis, at most
+  uint32_t many_tiles;  // 128-row tiles of the other requests, at most (0: none expected)
+  uint32_t many_splits;
+  uint64_t few_part;    // rows of partial results of the few-row requests,
+  uint64_t part_rows;   // and of all (hd + 2 floats each)
+};
+PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv, uint32_t hd, uint32_t max_q,
+                              uint32_t max_kv);
+
 struct PagedAttnArgs {
   const uint16_t* q;         // [n, hq, hd]; strides of a row and of a head
   uint64_t q_stride, q_head_stride;
@@ -64,6 +78,9 @@ struct PagedAttnArgs {
   uint32_t n, B, hq, hkv, hd, num_pages, page_shift, width;
   float scale;
   uint32_t elem;
+  PagedAttnPlan plan;        // GPU: how the work is split, and the splits' partial results
+  float* part_o;
+  float* part_ml;
 };
 
 struct VerifyArgs {

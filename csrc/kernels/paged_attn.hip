@@ -1,8 +1,32 @@
 // Attention of new tokens over a paged KV cache:
 //   o_i = sum_{t <= pos_i} softmax_t(scale q_i . k_t) v_t,   pos_i = kv - n + i
 // for row i of a request with n new rows and kv cached tokens (the new ones
-// among them).
+// among them). One pass over the keys with a running maximum m and sum l; both
+// products on the matrix cores.
+//
+// Layout of the two products. A request's rows of one kv head are its new
+// tokens times the g query heads of the group (row r: token r / g, head r % g),
+// so a key is read once for all of them. The scores are computed transposed,
+// S^T = K Q^T (A: 16 or 32 keys, B: 16 or 32 rows), because then
+//   - a lane owns ONE row: its maximum, sum and rescaling are per-lane values,
+//     and a row's keys lie in its own registers and one or three other lanes';
+//   - the accumulator's registers ARE the B operand of O^T = V^T P^T: an MFMA
+//     contracts over keys in any order as long as A and B agree, so P goes
+//     from the first product's accumulator into the second without a shuffle,
+//     and V^T is read from LDS in the same key order by the transposing LDS
+//     read (a 4 x 16 tile per 16 lanes).
+// K and V rows go global -> registers -> LDS (the next tile's loads fly while
+// this one is multiplied).
+//
+// Two bodies. `few` (up to 16 NB rows per kv head: single tokens, drafts) is
+// bound by the KV bytes: each wave streams its own 32-key blocks through
+// wave-private LDS without barriers, the waves join at the end. `many` (prompt
+// chunks) is bound by the matrix cores: four waves of 32 rows share each
+// 64-key tile. One launch serves both kinds in a mixed batch. The key axis is
+// split where rows are few; k_paged_combine joins the parts.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "ogkm/elem.hpp"
 #include "ogkm/kernels.hpp"
@@ -10,96 +34,807 @@
 
 namespace ogkm {
 
-// One wave per (row, query head): a lane scores one of 64 keys at a time, then
-// the wave adds the keys' value rows, two dims per lane. Running maximum and
-// sum in f32.
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
 template <typename T>
-__global__ void __launch_bounds__(256) k_paged_attn(PagedAttnArgs a) {
-  __shared__ float qs[4][128];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t item = blockIdx.x * 4 + wave;
-  const uint32_t t = item / a.hq, h = item - t * a.hq;
-  if (t >= a.n) return;
-  uint32_t lo = 0, hi = a.B;
-  while (lo < hi) {  // first request that ends behind row t
-    const uint32_t mid = (lo + hi) >> 1;
-    if (a.cu_q[mid + 1] > (int32_t)t)
-      hi = mid;
-    else
-      lo = mid + 1;
+struct Mma;
+template <>
+struct Mma<__bf16> {
+  typedef Vec<__bf16>::v8 v8;
+  static constexpr uint32_t kExp = 0x7F807F80u, kOne = 0x00800080u;  // exponent bits of a pair, their lowest
+  static __device__ __forceinline__ f32x4_t m16(u32x4 a, u32x4 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
-  if (lo == a.B || a.cu_q[lo] > (int32_t)t) return;
-  const uint32_t b = lo;
-  const int32_t n = min(a.cu_q[b + 1], (int32_t)a.n) - a.cu_q[b];
-  const int32_t kv = max(a.kv_lens[b], 0);
-  const int64_t pos = (int64_t)kv - n + ((int32_t)t - a.cu_q[b]);
-  const uint64_t kvh = h / (a.hq / a.hkv);
-  const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_stride + h * a.q_head_stride;
-  for (uint32_t d = lane; d < a.hd; d += 64) qs[wave][d] = to_f32<T>(q[d]) * a.scale;
-  __builtin_amdgcn_wave_barrier();
-  const int32_t* row = a.table + b * a.table_ld;
-  const T* k0 = reinterpret_cast<const T*>(a.pages) + kvh * a.head_stride;
-  const uint32_t mask = (1u << a.page_shift) - 1;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  bool bad = kv > ((int64_t)a.width << a.page_shift);
-  for (int64_t base = 0; base <= pos && !bad; base += 64) {
-    const int64_t key = base + lane;
-    float sc = -INFINITY;
-    uint64_t off = 0;
-    bool miss = false;
-    if (key <= pos) {
-      const int32_t page = row[key >> a.page_shift];
-      miss = page < 0 || (uint32_t)page >= a.num_pages;
-      if (!miss) {
-        off = page * a.page_stride + (key & mask) * a.hd;
-        sc = 0.f;
-        for (uint32_t d = 0; d < a.hd; ++d) sc += qs[wave][d] * to_f32<T>(k0[off + d]);
+  static __device__ __forceinline__ f32x16_t m32(u32x4 a, u32x4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<_Float16> {
+  typedef Vec<_Float16>::v8 v8;
+  static constexpr uint32_t kExp = 0x7C007C00u, kOne = 0x04000400u;
+  static __device__ __forceinline__ f32x4_t m16(u32x4 a, u32x4 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16_t m32(u32x4 a, u32x4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+
+// P is kept as 2^kShift p: an fp16 probability below 2^-14 would lose bits as a
+// subnormal (bf16 has f32's range); with it that begins at 2^-22. The sum
+// carries the same factor.
+template <typename T>
+constexpr float kShift = 0.f;
+template <>
+constexpr float kShift<_Float16> = 8.f;
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typename Vec<T>::v2 v = {from_f32<T>(a), from_f32<T>(b)};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// Any infinity or NaN among 8 elements?
+template <typename T>
+__device__ __forceinline__ bool nonfinite(u32x4 x) {
+  uint32_t hit = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) hit |= (x[j] & Mma<T>::kExp) + Mma<T>::kOne;
+  return (hit & 0x80008000u) != 0;
+}
+
+// V with infinities or NaNs in a tile that some row does not see whole: there a
+// probability of 0 times such a value would be NaN. Such a value is taken out
+// of V, and the first key that has one is kept for each dim and kind (NaN, +inf,
+// -inf) in LDS: a row sees keys 0 .. pos, so it sees one exactly if pos is not
+// before that key, and special() adds what it does to the row's sum.
+constexpr int32_t kNever = INT32_MAX;
+template <typename T, int HD>
+__device__ __forceinline__ void take_special(u32x4& x, int32_t key, uint32_t dim, int32_t* first_key) {
+  constexpr uint32_t inf = Mma<T>::kExp & 0xFFFFu;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int s = 0; s < 32; s += 16) {
+      const uint32_t v = (x[j] >> s) & 0xFFFFu;
+      if ((v & inf) == inf) {
+        const uint32_t kind = (v & 0x7FFFu) > inf ? 0u : v == inf ? 1u : 2u;
+        atomicMin(first_key + kind * HD + dim + 2 * j + s / 16, key);  // LDS, integers: the order does not matter
+        x[j] &= ~(0xFFFFu << s);
       }
     }
-    bad = __any(miss);
-    if (bad) break;
-    float mx = sc;
+}
+template <int HD>
+__device__ __forceinline__ float special(float o, int32_t pos, uint32_t dim, const int32_t* first_key) {
+  if (pos >= first_key[dim]) o = __builtin_nanf("");
+  if (pos >= first_key[HD + dim]) o += __builtin_inff();
+  if (pos >= first_key[2 * HD + dim]) o -= __builtin_inff();
+  return o;
+}
+
+// The 4 x 16 transposing LDS read: lane i of 16 gives the address of row i / 4,
+// elements 4 (i % 4) .. + 3, and gets column i of the four rows.
+__device__ __forceinline__ u32x2 read_tr(const uint16_t* p) {
+  const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+  return __builtin_bit_cast(u32x2, v);
+}
+
+// LDS rows are padded instead of swizzled: every access is then one lane
+// address plus a constant that fits the instruction, where XOR-ed chunks cost
+// the compiler an address register each (122 spilled registers in the 32-row
+// body). K: 16 bytes, the 8 lanes of a read phase take one chunk of 8 rows; V:
+// 32 bytes, a transposing read takes 32 bytes of 4 rows. Both touch every bank
+// once.
+template <int HD>
+constexpr int kKRow = HD + 8;
+template <int HD>
+constexpr int kVRow = HD + 16;
+template <int HD>
+constexpr int kKVRow = kKRow<HD> + kVRow<HD>;  // elements of LDS per key
+
+// The wave's number, known to the compiler as uniform: bounds, page ids and
+// addresses that follow from it stay in scalar registers.
+__device__ __forceinline__ uint32_t wave_id() { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
+struct Request {
+  int32_t row0, n;       // first row in q, new rows
+  int32_t kv, cap;       // cached tokens; kv > cap: the table row is too short
+};
+__device__ __forceinline__ Request request_of(const PagedAttnArgs& a, uint32_t b) {
+  Request r;
+  r.row0 = min(max(a.cu_q[b], 0), (int32_t)a.n);
+  r.n = min(max(a.cu_q[b + 1], r.row0), (int32_t)a.n) - r.row0;
+  r.kv = max(a.kv_lens[b], 0);
+  r.cap = (int32_t)(a.width << a.page_shift);
+  return r;
+}
+
+// Keys of one split: whole blocks of 32, at least kMinSplit keys, so that short
+// requests use few of the launch's splits.
+constexpr int32_t kMinSplit = 256;
+__device__ __forceinline__ int32_t split_keys(int32_t kv, uint32_t splits) {
+  const int32_t per = (int32_t)(((uint32_t)kv + splits - 1) / splits);
+  return max((per + 31) & ~31, kMinSplit);
+}
+__device__ __forceinline__ int32_t splits_used(int32_t kv, int32_t per) { return max((kv + per - 1) / per, 1); }
+
+// ---------------------------------------------------------------- few rows
+constexpr int kFewWaves = 4;
+
+template <typename T, int HD, int NB>
+__device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, uint32_t b, uint32_t kvh, uint32_t split) {
+  constexpr int KS = HD / 32, DT = HD / 16, LD = HD / 32;  // k steps, dim tiles, loads per 16 rows
+  constexpr int R = 16 * NB;
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id();
+  const uint32_t col = lane & 15, quad = lane >> 4;
+  const uint32_t g = a.hq / a.hkv;
+  const Request rq = request_of(a, b);
+  const int32_t rows = rq.n * (int32_t)g;
+  if (rows == 0 || rows > (int32_t)a.plan.few_rows) return;
+  const bool looped = rows > R;  // more rows than the host's bound: tile after tile, unsplit
+  const int32_t kv = rq.kv > rq.cap ? 0 : rq.kv;
+  const int32_t per = looped ? max(kv, 1) : split_keys(kv, a.plan.few_splits);
+  const int32_t used = looped ? 1 : splits_used(kv, per);
+  if ((int32_t)split >= used) return;
+  const int32_t c0 = (int32_t)split * per, c1 = min(c0 + per, kv);
+  // this wave's K block, then its V block; the lane's places in them
+  uint16_t* kw = lds + wave * (32 * kKVRow<HD>) + (lane / (HD / 8)) * kKRow<HD> + (lane % (HD / 8)) * 8;
+  uint16_t* vw = lds + wave * (32 * kKVRow<HD>) + 32 * kKRow<HD> + (lane / (HD / 8)) * kVRow<HD> + (lane % (HD / 8)) * 8;
+  const uint16_t* kread = lds + wave * (32 * kKVRow<HD>) + col * kKRow<HD> + 8 * quad;
+  const uint16_t* vread = lds + wave * (32 * kKVRow<HD>) + 32 * kKRow<HD> + (4 * quad + (col >> 2)) * kVRow<HD> + 4 * (col & 3);
+  __shared__ float wm[kFewWaves][R], wl[kFewWaves][R];
+  __shared__ int32_t first_key[kFewWaves][3 * HD];  // take_special; set only by a wave that met one
+  __shared__ uint32_t special_s[kFewWaves];
+  const uint16_t* kbase = a.pages + kvh * a.head_stride;
+  const int32_t* table = a.table + b * a.table_ld;
+  const float c = a.scale * 1.44269504088896340736f;  // scores in powers of two
+  const int32_t blocks = (c1 - c0 + 31) >> 5;
+
+  for (int32_t tile0 = 0; tile0 < rows; tile0 += R) {
+    // this lane's rows, one per column block: the B operand and the last key each sees
+    u32x4 qf[NB][KS];
+    int32_t pos[NB];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    const float mn = fmaxf(m, mx);
-    const float f = m == -INFINITY ? 0.f : __expf(m - mn);
-    const float p = key <= pos ? __expf(sc - mn) : 0.f;
-    float ps = p;
+    for (int nb = 0; nb < NB; ++nb) {
+      const int32_t r = tile0 + nb * 16 + (int32_t)col;
+      const bool in = r < rows;
+      const uint32_t tok = in ? (uint32_t)r / g : 0u, h = in ? (uint32_t)r - tok * g : 0u;
+      pos[nb] = in ? rq.kv - rq.n + (int32_t)tok : rq.kv - 1;
+      const uint16_t* q = a.q + (uint64_t)(rq.row0 + tok) * a.q_stride + (kvh * g + h) * a.q_head_stride + 8 * quad;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) ps += __shfl_xor(ps, o, 64);
-    l = l * f + ps;
-    o0 *= f;
-    o1 *= f;
-    m = mn;
-    const int cnt = pos - base + 1 < 64 ? (int)(pos - base + 1) : 64;
-    for (int j = 0; j < cnt; ++j) {
-      const float pj = __shfl(p, j, 64);
-      const uint64_t oj = __shfl(off, j, 64);
-      const T* v = k0 + a.kv_stride + oj;
-      if (2 * lane < a.hd) {
-        o0 += pj * to_f32<T>(v[2 * lane]);
-        o1 += pj * to_f32<T>(v[2 * lane + 1]);
+      for (int k = 0; k < KS; ++k) {
+        qf[nb][k] = *reinterpret_cast<const u32x4*>(q + 32 * k);
+        if (!in) qf[nb][k] = u32x4{0u, 0u, 0u, 0u};
       }
     }
-  }
-  if (2 * lane < a.hd) {
-    T* out = reinterpret_cast<T*>(a.out) + t * a.out_stride + (uint64_t)h * a.hd + 2 * lane;
-    const float none = bad ? __builtin_nanf("") : 0.f;
-    out[0] = from_f32<T>(bad || pos < 0 ? none : o0 / l);
-    out[1] = from_f32<T>(bad || pos < 0 ? none : o1 / l);
+    // rows of this tile see keys up to here at least: blocks before it need no mask
+    const int32_t first = rq.kv - rq.n + tile0 / (int32_t)g;
+    f32x4_t o[NB][DT];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb] = -__builtin_inff();
+      l[nb] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[nb][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    bool wave_special = false;
+    // Page ids of this wave's next 32 blocks, one half block per lane (a page
+    // holds at least 16 tokens), so that a block's addresses are wave-uniform.
+    int32_t ids = 0;
+    auto fetch_ids = [&](int32_t n0) {
+      const int32_t t = c0 + ((n0 + (int32_t)(lane >> 1)) * kFewWaves + (int32_t)wave) * 32 + 16 * (int32_t)(lane & 1);
+      ids = t < c1 ? table[t >> a.page_shift] : 0;
+    };
+    u32x4 kr[2 * LD], vr[2 * LD];
+    bool miss0 = false, miss1 = false, next0 = false, next1 = false;
+    auto load = [&](int32_t n) {
+      const int32_t t0 = c0 + (n * kFewWaves + (int32_t)wave) * 32;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int32_t page = __builtin_amdgcn_readlane(ids, 2 * (n & 31) + h);
+        const bool miss = (uint32_t)page >= a.num_pages;
+        (h ? next1 : next0) = miss;
+        if (miss) page = 0;
+        const uint32_t row = (uint32_t)(t0 + 16 * h) & ((1u << a.page_shift) - 1u);
+        const uint16_t* src = kbase + (uint64_t)page * a.page_stride + (uint64_t)row * HD;
+#pragma unroll
+        for (int j = 0; j < LD; ++j) kr[h * LD + j] = *reinterpret_cast<const u32x4*>(src + (j * 64 + lane) * 8);
+#pragma unroll
+        for (int j = 0; j < LD; ++j)
+          vr[h * LD + j] = *reinterpret_cast<const u32x4*>(src + a.kv_stride + (j * 64 + lane) * 8);
+      }
+    };
+    const int32_t mine = (blocks - (int32_t)wave + kFewWaves - 1) / kFewWaves;
+    if (mine > 0) {
+      fetch_ids(0);
+      load(0);
+    }
+    for (int32_t n = 0; n < mine; ++n) {
+      const int32_t t0 = c0 + (n * kFewWaves + (int32_t)wave) * 32;
+      miss0 = next0;
+      miss1 = next1;
+      const bool masked = t0 + 31 > first;
+      bool odd = false;
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 2 * LD; ++j) odd |= nonfinite<T>(vr[j]);
+        if (__any(odd)) {
+          if (!wave_special)
+            for (uint32_t e = lane; e < 3 * HD; e += 64) first_key[wave][e] = kNever;
+          wave_special = true;
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int j = 0; j < 2 * LD; ++j)
+            take_special<T, HD>(vr[j], t0 + j * (512 / HD) + (int32_t)(lane / (HD / 8)), lane % (HD / 8) * 8, first_key[wave]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * LD; ++j) {  // 512 / HD rows by each wave-wide store
+        *reinterpret_cast<u32x4*>(kw + j * (512 / HD) * kKRow<HD>) = kr[j];
+        *reinterpret_cast<u32x4*>(vw + j * (512 / HD) * kVRow<HD>) = vr[j];
+      }
+      if (n + 1 < mine) {
+        if (((n + 1) & 31) == 0) fetch_ids(n + 1);
+        load(n + 1);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      // S^T: two tiles of 16 keys
+      f32x4_t s[2][NB];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s[t][nb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u32x4 ka = *reinterpret_cast<const u32x4*>(kread + t * 16 * kKRow<HD> + 32 * k);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) s[t][nb] = Mma<T>::m16(ka, qf[nb][k], s[t][nb]);
+        }
+      }
+      u32x4 p[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float x[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float v = s[t][nb][r] * c;
+            if (t ? miss1 : miss0) v = __builtin_nanf("");  // a page outside the pool
+            x[4 * t + r] = v;
+          }
+        if (masked) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (t0 + 16 * t + 4 * (int32_t)quad + r > pos[nb]) x[4 * t + r] = -__builtin_inff();
+        }
+        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mn = fmaxf(m[nb], mx);
+        if (__any(mn > m[nb])) {
+          const float f = m[nb] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[nb] - mn);
+          // a row that saw only -inf so far has l = 0 or NaN: kept by l * 1
+          const float fl = m[nb] == mn ? 1.f : f;
+          l[nb] *= fl;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[nb][d] *= fl;
+          m[nb] = mn;
+        }
+        const float base = (mn == -__builtin_inff() ? 0.f : mn) - kShift<T>;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = __builtin_amdgcn_exp2f(x[j] - base);
+          l[nb] += x[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[nb][j] = pack2<T>(x[2 * j], x[2 * j + 1]);
+      }
+      // O^T += V^T P^T, keys in the order of P's registers: 4 quad .. + 3 of each 16-key tile
+      auto v_frag = [&](int d) {
+        const u32x2 lo = read_tr(vread + 16 * d), hi = read_tr(vread + 16 * kVRow<HD> + 16 * d);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+      };
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const u32x4 va = v_frag(d);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) o[nb][d] = Mma<T>::m16(va, p[nb], o[nb][d]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    // Join the waves: maxima through LDS, then two rounds of adding halves
+    // (waves 2, 3 -> 0, 1; wave 1 -> 0), f32 in the K / V space.
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      l[nb] += __shfl_xor(l[nb], 16, 64);
+      l[nb] += __shfl_xor(l[nb], 32, 64);
+      if (quad == 0) {
+        wm[wave][nb * 16 + col] = m[nb];
+        wl[wave][nb * 16 + col] = l[nb];
+      }
+    }
+    if (lane == 0) special_s[wave] = wave_special;
+    __syncthreads();  // also: every wave is done with its blocks
+    float big[NB], sum[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t r = nb * 16 + col;
+      big[nb] = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+      sum[nb] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w) {
+        const float f = wm[w][r] == -__builtin_inff() ? (big[nb] == wm[w][r] ? 1.f : 0.f)
+                                                      : __builtin_amdgcn_exp2f(wm[w][r] - big[nb]);
+        sum[nb] += f * wl[w][r];
+        if ((uint32_t)w == wave)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[nb][d] *= f;
+      }
+    }
+    float* ox = reinterpret_cast<float*>(lds);  // [2][R][HD]; the lanes' own order, 16 bytes each
+    auto put = [&](float* at) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_t*>(at + ((nb * DT + d) * 64 + lane) * 4) = o[nb][d];
+    };
+    auto add = [&](const float* at) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[nb][d] += *reinterpret_cast<const f32x4_t*>(at + ((nb * DT + d) * 64 + lane) * 4);
+    };
+    if (wave >= 2) put(ox + (wave - 2) * R * HD);
+    __syncthreads();
+    if (wave < 2) add(ox + wave * R * HD);
+    __syncthreads();
+    if (wave == 1) put(ox);
+    __syncthreads();
+    if (wave == 0) {
+      add(ox);
+      for (int w = 0; w < kFewWaves; ++w)
+        if (special_s[w])
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nb][d][e] = special<HD>(o[nb][d][e], pos[nb], 16 * d + 4 * quad + e, first_key[w]);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int32_t r = tile0 + nb * 16 + (int32_t)col;
+        if (r >= rows) continue;
+        const uint32_t tok = (uint32_t)r / g, h = (uint32_t)r - tok * g;
+        if (used == 1) {
+          float inv = 1.f / sum[nb];
+          if (rq.kv > rq.cap) inv = __builtin_nanf("");
+          uint16_t* dst = a.out + (uint64_t)(rq.row0 + tok) * a.out_stride + (uint64_t)(kvh * g + h) * HD + 4 * quad;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            f32x4_t v = o[nb][d];
+            // a row that sees nothing is 0; 0 / 0 of a row that saw only -inf is NaN
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = pos[nb] < 0 && rq.kv <= rq.cap ? 0.f : sum[nb] == 0.f ? __builtin_nanf("") : v[e] * inv;
+            *reinterpret_cast<u32x2*>(dst + 16 * d) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+          }
+        } else {
+          const uint64_t at = (((uint64_t)b * a.hkv + kvh) * a.plan.few_splits + split) * R + nb * 16 + col;
+          if (quad == 0) {
+            a.part_ml[2 * at] = big[nb];
+            a.part_ml[2 * at + 1] = sum[nb];
+          }
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            *reinterpret_cast<f32x4_t*>(a.part_o + at * HD + 16 * d + 4 * quad) = o[nb][d];
+        }
+      }
+    }
+    if (looped) __syncthreads();  // the next tile writes the LDS again
   }
 }
 
-hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t s) {
-  if (!a.hkv || a.hq % a.hkv || (a.hd != 64 && a.hd != 128) || a.page_shift > 16) return hipErrorInvalidValue;
-  const uint64_t waves = (uint64_t)a.n * a.hq;
-  if (!waves || !a.B) return hipSuccess;
-  const dim3 grid((uint32_t)((waves + 3) / 4));
-  if (a.elem == ELEM_F16)
-    hipLaunchKernelGGL((k_paged_attn<_Float16>), grid, dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_paged_attn<__bf16>), grid, dim3(256), 0, s, a);
+// ---------------------------------------------------------------- many rows
+constexpr int kManyRows = 128;  // rows of a workgroup's tile: 4 waves of 32
+constexpr int kManyKeys = 64;   // keys of a K / V tile
+
+// Tile x of all tiles of the requests with more than few_rows rows, the last
+// request's last tile first (of a prompt's tiles the last sees the most keys).
+// Every wave scans the request lengths by itself. Returns false past the end.
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, uint32_t x, uint32_t* b, int32_t* tile) {
+  const uint32_t lane = threadIdx.x & 63;
+  const int32_t g = (int32_t)(a.hq / a.hkv);
+  for (int32_t top = (int32_t)a.B; top > 0; top -= 64) {  // lane: request top - 1 - lane
+    const int32_t r = top - 1 - (int32_t)lane;
+    uint32_t tiles = 0;
+    if (r >= 0) {
+      const int32_t lo = min(max(a.cu_q[r], 0), (int32_t)a.n), hi = min(max(a.cu_q[r + 1], lo), (int32_t)a.n);
+      const uint32_t rows = (uint32_t)(hi - lo) * (uint32_t)g;
+      tiles = rows > a.plan.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
+    }
+    uint32_t upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = __shfl_up(upto, o, 64);
+      if ((int)lane >= o) upto += y;
+    }
+    const uint64_t past = __ballot(upto > x);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      *b = (uint32_t)(top - 1 - l);
+      *tile = (int32_t)((uint32_t)__builtin_amdgcn_readlane((int)upto, l) - 1 - x);
+      return true;
+    }
+    x -= (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  }
+  return false;
+}
+
+// Raise of a row's running maximum (in powers of two) that the accumulators do
+// not follow: probabilities may reach 2^kLazy, and rescaling O becomes rare
+// after the first tiles. fp16: 2^(kLazy + shift) stays below 65504.
+constexpr float kLazy = 6.f;
+
+template <typename T, int HD>
+__device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds, uint32_t x, uint32_t kvh, uint32_t split) {
+  constexpr int KS = HD / 16, DT = HD / 32;        // k steps, 32-dim tiles
+  constexpr int LJ = kManyKeys * HD / 8 / 256;     // 16-byte loads of a thread per tile and tensor
+  constexpr uint32_t kTile = kManyKeys * kKVRow<HD>;  // LDS elements of a K and V tile
+  constexpr uint32_t kV = kManyKeys * kKRow<HD>;      // where its V begins
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id(), tid = threadIdx.x;
+  const uint32_t col = lane & 31, half = lane >> 5;
+  const uint32_t g = a.hq / a.hkv;
+  uint32_t b;
+  int32_t ti;
+  if (!find_tile(a, x, &b, &ti)) return;
+  const Request rq = request_of(a, b);
+  const int32_t rows = rq.n * (int32_t)g, r0 = ti * kManyRows;
+  const bool bad = rq.kv > rq.cap;
+  // keys that any row of the tile sees, and this split's share
+  const int32_t last = rq.kv - rq.n + (min(r0 + kManyRows, rows) - 1) / (int32_t)g;
+  const int32_t kend = bad ? 0 : max(last + 1, 0);
+  const int32_t per = split_keys(kend, a.plan.many_splits), used = splits_used(kend, per);
+  if ((int32_t)split >= used) return;
+  const int32_t c0 = (int32_t)split * per, c1 = min(c0 + per, kend);
+  const uint16_t* kbase = a.pages + kvh * a.head_stride;
+  const int32_t* table = a.table + b * a.table_ld;
+  // scores in powers of two; the sign of the scale goes into q, so that the
+  // largest product is the largest score
+  const float c = fabsf(a.scale) * 1.44269504088896340736f;
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+
+  const int32_t r = r0 + (int32_t)(wave * 32 + col);
+  const bool in = r < rows;
+  const uint32_t tok = in ? (uint32_t)r / g : 0u, h = in ? (uint32_t)r - tok * g : 0u;
+  const int32_t pos = in ? rq.kv - rq.n + (int32_t)tok : last;
+  u32x4 qf[KS];
+  {
+    const uint16_t* q = a.q + (uint64_t)(rq.row0 + tok) * a.q_stride + (kvh * g + h) * a.q_head_stride + 8 * half;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      qf[k] = *reinterpret_cast<const u32x4*>(q + 16 * k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qf[k][j] = in ? qf[k][j] ^ flip : 0u;
+    }
+  }
+  // of this wave's rows: the fewest and the most keys seen
+  const int32_t w0 = r0 + (int32_t)wave * 32, w1 = min(w0 + 32, rows) - 1;
+  const int32_t wfirst = rq.kv - rq.n + w0 / (int32_t)g;
+  const int32_t wlast = w0 < rows ? rq.kv - rq.n + w1 / (int32_t)g : -1;
+
+  f32x16_t o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;  // m: what the accumulators are scaled by, in units of c
+
+  // the lane's places in a tile
+  const uint32_t kw = tid / (HD / 8) * kKRow<HD> + tid % (HD / 8) * 8, vw = kV + tid / (HD / 8) * kVRow<HD> + tid % (HD / 8) * 8;
+  const uint32_t kread = col * kKRow<HD> + 8 * half;
+  const uint32_t vread = kV + (4 * half + ((lane & 15) >> 2)) * kVRow<HD> + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const uint32_t mine = (tid / (HD / 8)) % 16 * HD + tid % (HD / 8) * 8;  // in its group of 16 keys
+
+  int32_t ids = 0;  // page of the lane's group of 16 keys, for 16 tiles
+  u32x4 kr[LJ], vr[LJ];
+  uint32_t next_miss = 0, miss = 0;  // groups of the tile whose page is outside the pool
+  auto load = [&](int32_t i) {
+    if ((i & 15) == 0) {
+      const int32_t t = c0 + i * kManyKeys + 16 * (int32_t)lane;
+      ids = t < c1 ? table[t >> a.page_shift] : 0;
+    }
+    const uint64_t out = __ballot((uint32_t)ids >= a.num_pages);
+    next_miss = (uint32_t)(out >> (4 * (i & 15))) & 15u;
+#pragma unroll
+    for (int j = 0; j < LJ; ++j) {
+      const uint32_t grp = (j * 256 + wave * 64) / (HD / 8) / 16;  // wave-uniform: 16 keys, one page
+      int32_t page = __builtin_amdgcn_readlane(ids, 4 * (i & 15) + grp);
+      if ((uint32_t)page >= a.num_pages) page = 0;
+      const uint32_t at = (uint32_t)(c0 + i * kManyKeys + 16 * (int32_t)grp) & ((1u << a.page_shift) - 1u);
+      const uint16_t* src = kbase + (uint64_t)page * a.page_stride + (uint64_t)at * HD;
+      kr[j] = *reinterpret_cast<const u32x4*>(src + mine);
+      vr[j] = *reinterpret_cast<const u32x4*>(src + a.kv_stride + mine);
+    }
+  };
+  const int32_t tiles = (c1 - c0 + kManyKeys - 1) / kManyKeys;
+  const int32_t first = rq.kv - rq.n + r0 / (int32_t)g;  // of the whole tile of rows
+  __shared__ int32_t first_key[3 * HD];  // take_special
+  __shared__ uint32_t special_s;
+  for (uint32_t e = tid; e < 3 * HD; e += 256) first_key[e] = kNever;
+  if (tid == 0) special_s = 0;
+  if (tiles > 0) load(0);
+  __syncthreads();
+  for (int32_t i = 0; i < tiles; ++i) {
+    const int32_t t0 = c0 + i * kManyKeys;
+    uint16_t* buf = lds + (i & 1) * kTile;
+    const bool tile_masked = t0 + kManyKeys - 1 > first;
+    if (tile_masked) {
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < LJ; ++j) odd |= nonfinite<T>(vr[j]);
+      if (odd) {
+        special_s = 1;
+#pragma unroll
+        for (int j = 0; j < LJ; ++j)
+          take_special<T, HD>(vr[j], t0 + j * (2048 / HD) + (int32_t)(tid / (HD / 8)), tid % (HD / 8) * 8, first_key);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < LJ; ++j) {
+      *reinterpret_cast<u32x4*>(buf + kw + j * (2048 / HD) * kKRow<HD>) = kr[j];
+      *reinterpret_cast<u32x4*>(buf + vw + j * (2048 / HD) * kVRow<HD>) = vr[j];
+    }
+    miss = next_miss;
+    if (i + 1 < tiles) load(i + 1);
+    // the other buffer's readers passed the barrier of the tile before
+    __syncthreads();
+    if (t0 > wlast) continue;  // none of this wave's rows sees the tile
+
+    f32x16_t s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        s[t] = Mma<T>::m32(*reinterpret_cast<const u32x4*>(buf + kread + t * 32 * kKRow<HD> + 16 * k), qf[k], s[t]);
+    }
+    // register e of s[t] is key 32 t + 8 (e / 4) + 4 half + e % 4
+    if (miss) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (miss >> (2 * t + e / 8) & 1) s[t][e] = __builtin_nanf("");
+    }
+    if (t0 + kManyKeys - 1 > wfirst) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (t0 + 32 * t + 8 * (e / 4) + 4 * (int32_t)half + e % 4 > pos) s[t][e] = -__builtin_inff();
+    }
+    float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(s[0][e], s[1][e]));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+    if (__any(mx > m + kLazy) || i == 0) {
+      const float mn = fmaxf(m, mx);
+      const float f = m == mn ? 1.f : m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+      m = mn;
+    }
+    const float base = (m == -__builtin_inff() ? 0.f : m) - kShift<T>;
+    u32x4 p[4];  // B operands of the four groups of 16 keys
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -base)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], c, -base));
+        l += p0 + p1;
+        p[2 * t + e / 8][(e % 8) / 2] = pack2<T>(p0, p1);
+      }
+    // V^T operand of dims 32 d .., keys 16 kt ..: two 16-dim halves by lane group
+    auto v_frag = [&](int d, int kt) {
+      const uint16_t* at = buf + vread + 16 * kt * kVRow<HD> + 32 * d;
+      const u32x2 lo = read_tr(at), hi = read_tr(at + 8 * kVRow<HD>);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] = Mma<T>::m32(v_frag(d, kt), p[kt], o[d]);
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!in) return;
+  if (tiles > 0 && special_s)  // set before the last tile's barrier
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        o[d][e] = special<HD>(o[d][e], pos, 32 * d + 8 * (e / 4) + 4 * half + e % 4, first_key);
+  if (used == 1) {
+    const float inv = 1.f / l;
+    uint16_t* dst = a.out + (uint64_t)(rq.row0 + tok) * a.out_stride + (uint64_t)(kvh * g + h) * HD + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[j] = bad || (l == 0.f && pos >= 0) ? __builtin_nanf("") : pos < 0 ? 0.f : o[d][e + j] * inv;
+        *reinterpret_cast<u32x2*>(dst + 32 * d + 2 * e) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+      }
+  } else {
+    const uint64_t at = a.plan.few_part + (((uint64_t)x * a.hkv + kvh) * a.plan.many_splits + split) * kManyRows + wave * 32 + col;
+    if (half == 0) {
+      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at + 1] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<f32x4_t*>(a.part_o + at * HD + 32 * d + 2 * e + 4 * half) =
+            f32x4_t{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+  }
+}
+
+template <typename T, int HD, int NB>
+__global__ void __launch_bounds__(64 * kFewWaves, NB == 4 ? 1 : 2) k_paged_few(PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kFewWaves * 32 * kKVRow<HD>];
+  few_body<T, HD, NB>(a, lds, blockIdx.z, blockIdx.x, blockIdx.y);
+}
+
+// Both kinds of requests in one launch: the long tiles first, then the few-row
+// requests, which fill in beside them.
+template <typename T, int HD, int NB>
+__global__ void __launch_bounds__(256, NB == 4 ? 1 : 2) k_paged_mixed(PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kManyKeys * kKVRow<HD>];
+  uint32_t i = blockIdx.x;
+  const uint32_t kvh = i % a.hkv;  // a head's workgroups share their K and V, and with 8 heads an XCD's L2
+  i /= a.hkv;
+  const uint32_t many = a.plan.many_tiles * a.plan.many_splits;
+  if (i < many) {
+    many_body<T, HD>(a, lds, i / a.plan.many_splits, kvh, i % a.plan.many_splits);
+  } else {
+    i -= many;
+    few_body<T, HD, NB>(a, lds, i / a.plan.few_splits, kvh, i % a.plan.few_splits);
+  }
+}
+
+// Joins the splits of a row: one wave per row, HD / 64 dims a lane. The first
+// many_tiles blocks of rows are those of the tiles, then each request's few rows.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) k_paged_combine(PagedAttnArgs a) {
+  constexpr int E = HD / 64;
+  const uint32_t lane = threadIdx.x & 63, kvh = blockIdx.y;
+  const uint32_t g = a.hq / a.hkv;
+  const uint32_t many_groups = a.plan.many_splits > 1 ? a.plan.many_tiles * (kManyRows / 4) : 0;
+  uint32_t b, splits, R;
+  int32_t r, keys;  // row of the request, keys that were split
+  uint64_t at;
+  Request rq;
+  if (blockIdx.x < many_groups) {
+    const uint32_t x = blockIdx.x / (kManyRows / 4), rr = (blockIdx.x % (kManyRows / 4)) * 4 + wave_id();
+    int32_t ti;
+    if (!find_tile(a, x, &b, &ti)) return;
+    rq = request_of(a, b);
+    const int32_t rows = rq.n * (int32_t)g, r0 = ti * kManyRows;
+    r = r0 + (int32_t)rr;
+    if (r >= rows) return;
+    keys = max(rq.kv - rq.n + (min(r0 + kManyRows, rows) - 1) / (int32_t)g + 1, 0);
+    splits = a.plan.many_splits;
+    R = kManyRows;
+    at = a.plan.few_part + ((uint64_t)x * a.hkv + kvh) * splits * R + rr;
+  } else {
+    const uint32_t i = blockIdx.x - many_groups;
+    R = 16 * a.plan.few_blocks;
+    b = i / (R / 4);
+    const uint32_t rr = (i % (R / 4)) * 4 + wave_id();
+    rq = request_of(a, b);
+    const int32_t rows = rq.n * (int32_t)g;
+    r = (int32_t)rr;
+    if (r >= rows || rows > (int32_t)R) return;
+    keys = rq.kv;
+    splits = a.plan.few_splits;
+    at = ((uint64_t)b * a.hkv + kvh) * splits * R + rr;
+  }
+  if (rq.kv > rq.cap) return;
+  const int32_t used = splits_used(keys, split_keys(keys, splits));
+  if (used == 1) return;
+  float big = -__builtin_inff();
+  for (int32_t s = 0; s < used; ++s) big = fmaxf(big, a.part_ml[2 * (at + (uint64_t)s * R)]);
+  float sum = 0.f, o[E] = {};
+#pragma unroll 4
+  for (int32_t s = 0; s < used; ++s) {
+    const uint64_t i = at + (uint64_t)s * R;
+    const float m = a.part_ml[2 * i];
+    const float f = m == -__builtin_inff() ? (big == m ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - big);
+    sum += f * a.part_ml[2 * i + 1];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += f * a.part_o[i * HD + lane * E + e];
+  }
+  const uint32_t tok = (uint32_t)r / g, h = (uint32_t)r - tok * g;
+  const bool none = rq.kv - rq.n + (int32_t)tok < 0;
+  T* out = reinterpret_cast<T*>(a.out) + (uint64_t)(rq.row0 + tok) * a.out_stride + (uint64_t)(kvh * g + h) * HD;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[lane * E + e] = from_f32<T>(none ? 0.f : o[e] / sum);
+}
+
+template <typename T, int HD, int NB>
+hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t s) {
+  const PagedAttnPlan& p = a.plan;
+  if (p.many_tiles) {
+    const uint64_t wgs = ((uint64_t)p.many_tiles * p.many_splits + (uint64_t)a.B * p.few_splits) * a.hkv;
+    if (wgs > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_paged_mixed<T, HD, NB>), dim3((uint32_t)wgs), dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((k_paged_few<T, HD, NB>), dim3(a.hkv, p.few_splits, a.B), dim3(64 * kFewWaves), 0, s, a);
+  }
+  const uint64_t groups = (p.many_splits > 1 ? (uint64_t)p.many_tiles * (kManyRows / 4) : 0) +
+                          (p.few_splits > 1 ? (uint64_t)a.B * 4 * NB : 0);
+  if (groups > INT32_MAX) return hipErrorInvalidValue;
+  if (groups) hipLaunchKernelGGL((k_paged_combine<T, HD>), dim3((uint32_t)groups, a.hkv), dim3(256), 0, s, a);
   return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_attn_of(const PagedAttnArgs& a, hipStream_t s) {
+#define OGKM_ATTN_NB(HD)                                              \
+  (a.plan.few_blocks == 1   ? launch_attn<T, HD, 1>(a, s)             \
+   : a.plan.few_blocks == 2 ? launch_attn<T, HD, 2>(a, s)             \
+                            : launch_attn<T, HD, 4>(a, s))
+  return a.hd == 128 ? OGKM_ATTN_NB(128) : OGKM_ATTN_NB(64);
+#undef OGKM_ATTN_NB
+}
+
+}  // namespace
+
+PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv, uint32_t hd, uint32_t max_q,
+                              uint32_t max_kv) {
+  PagedAttnPlan p{};
+  const uint64_t g = hq / hkv, most = std::min(max_q, n) * g;  // rows of a request, at most
+  const uint64_t heads = hkv, key_splits = std::max<uint64_t>((max_kv + kMinSplit - 1) / kMinSplit, 1);
+  const uint64_t few = most <= 64 ? most : g;  // rows that the few-row body is laid out for
+  p.few_blocks = few <= 16 ? 1 : few <= 32 ? 2 : 4;
+  p.many_splits = 1;
+  if (most <= 64) {
+    p.few_rows = INT32_MAX;  // a request beyond the host's bound is taken tile by tile
+  } else {
+    // 0 rows where one token already fills the tiles
+    p.few_rows = g <= 64 ? 16 * p.few_blocks : 0;
+    p.many_tiles = (uint32_t)(n * g / kManyRows + std::min<uint64_t>(B, n * g / (p.few_rows + 1)));
+    const uint64_t wgs = std::max<uint64_t>(p.many_tiles * heads, 1);
+    p.many_splits = (uint32_t)std::min<uint64_t>((512 + wgs - 1) / wgs, key_splits);
+  }
+  const uint64_t wgs = std::max<uint64_t>(B * heads, 1);
+  p.few_splits = (uint32_t)std::min<uint64_t>((1024 + wgs - 1) / wgs, key_splits);
+  p.few_part = p.few_splits > 1 ? wgs * p.few_splits * 16 * p.few_blocks : 0;
+  p.part_rows = p.few_part + (p.many_splits > 1 ? p.many_tiles * heads * p.many_splits * kManyRows : 0);
+  return p;
+}
+
+hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t s) {
+  if (!a.hkv || a.hq % a.hkv || (a.hd != 64 && a.hd != 128) || a.page_shift < 4 || a.page_shift > 8 || !a.plan.few_splits ||
+      a.hkv > 65535 || a.plan.few_splits > 65535 || a.B > 65535)
+    return hipErrorInvalidValue;
+  if (!a.n || !a.B) return hipSuccess;
+  return a.elem == ELEM_F16 ? launch_attn_of<_Float16>(a, s) : launch_attn_of<__bf16>(a, s);
 }
 
 }  // namespace ogkm

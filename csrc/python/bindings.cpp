@@ -1168,19 +1168,31 @@ PYBIND11_MODULE(_ogkm, m) {
                          uint64_t pages, uint64_t kv_stride, uint64_t page_stride, uint64_t head_stride, uint64_t cu_q,
                          uint64_t kv_lens, uint64_t table, uint64_t table_ld, uint64_t out, uint64_t out_stride,
                          uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv, uint32_t hd, uint32_t num_pages,
-                         uint32_t page_size, uint32_t width, float scale, uint32_t elem) {
+                         uint32_t page_size, uint32_t width, float scale, uint32_t elem, uint32_t max_q,
+                         uint32_t max_kv, uint64_t part, uint64_t part_bytes) {
     const uint32_t shift = page_shift_of(page_size, "paged_attn");
+    if (B > 65535 || hkv > 65535 || (uint64_t)width * page_size > (1u << 30))
+      throw StatusError("paged_attn: at most 65535 requests and kv heads, 2^30 tokens per request");
     if (!hkv || hq % hkv || (hd != 64 && hd != 128) || elem > ELEM_F16 || n > INT32_MAX)
       throw StatusError("paged_attn: hq % hkv, hd 64 or 128, bf16 or fp16");
     PagedAttnArgs a{(const uint16_t*)q, q_stride, q_head_stride, (const uint16_t*)pages, kv_stride, page_stride,
                     head_stride, (const int32_t*)cu_q, (const int32_t*)kv_lens, (const int32_t*)table, table_ld,
-                    (uint16_t*)out, out_stride, n, B, hq, hkv, hd, num_pages, shift, width, scale, elem};
+                    (uint16_t*)out, out_stride, n, B, hq, hkv, hd, num_pages, shift, width, scale, elem,
+                    paged_attn_plan(n, B, hq, hkv, hd, max_q, max_kv), nullptr, nullptr};
+    if (!rt()->be()->is_fake() && a.plan.part_rows * (hd + 2) * 4 > part_bytes) throw StatusError("paged_attn: partial workspace too small");
+    a.part_o = (float*)part;
+    a.part_ml = (float*)part + a.plan.part_rows * hd;
     check(rt()->be()->paged_attn(dev, a, (void*)stream), "paged_attn");
   }, py::arg("dev"), py::arg("stream"), py::arg("q"), py::arg("q_stride"), py::arg("q_head_stride"),
      py::arg("pages"), py::arg("kv_stride"), py::arg("page_stride"), py::arg("head_stride"), py::arg("cu_q"),
      py::arg("kv_lens"), py::arg("table"), py::arg("table_ld"), py::arg("out"), py::arg("out_stride"), py::arg("n"),
      py::arg("B"), py::arg("hq"), py::arg("hkv"), py::arg("hd"), py::arg("num_pages"), py::arg("page_size"),
-     py::arg("width"), py::arg("scale"), py::arg("elem"));
+     py::arg("width"), py::arg("scale"), py::arg("elem"), py::arg("max_q"), py::arg("max_kv"), py::arg("part"),
+     py::arg("part_bytes"));
+  m.def("paged_attn_workspace", [](uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv, uint32_t hd, uint32_t max_q,
+                                   uint32_t max_kv) {  // bytes
+    return hkv ? paged_attn_plan(n, B, hq, hkv, hd, max_q, max_kv).part_rows * (hd + 2) * 4 : 0;
+  }, py::arg("n"), py::arg("B"), py::arg("hq"), py::arg("hkv"), py::arg("hd"), py::arg("max_q"), py::arg("max_kv"));
   m.def("verify_chunk", [] { return kVerifyChunk; });
   m.def("verify_draft", [](int dev, uint64_t stream, uint64_t p, uint64_t p_batch, uint64_t p_row, uint64_t q,
                            uint64_t q_batch, uint64_t q_row, uint64_t tokens, uint64_t u, uint64_t u_last,

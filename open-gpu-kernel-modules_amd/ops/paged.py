@@ -185,16 +185,27 @@ def attention(q: torch.Tensor, pages: torch.Tensor, cu_q: torch.Tensor, kv_lens:
     _ints("attention", "cu_q", cu_q, (B + 1,))
     _table("attention", block_table, B)
     width = block_table.shape[1]
-    if width * size >= 2**31:
-        raise ValueError("attention: positions below 2^31")
+    if width * size > 2**30 or B > 65535 or hkv > 65535:
+        raise ValueError("attention: at most 2^30 tokens per request, 65535 requests and kv heads")
+    max_q = n if max_q is None else min(max(int(max_q), 1), n)
+    max_kv = width * size if max_kv is None else min(max(int(max_kv), 1), width * size)
     if out is None:
         out = torch.empty(n, hq * hd, dtype=q.dtype, device=q.device)
     elif out.dtype != q.dtype or tuple(out.shape) != (n, hq * hd) or out.stride(1) != 1 or (
             n > 1 and (out.stride(0) % 8 or out.stride(0) < hq * hd)) or out.data_ptr() % 16:
         raise ValueError(f"attention: out must be {q.dtype} [{n}, {hq * hd}] with contiguous, aligned rows")
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    if not 1e-30 < abs(scale) < 1e30:
+        raise ValueError(f"attention: scale {scale}")
     dev, stream = _where("attention", q, pages=pages, cu_q=cu_q, kv_lens=kv_lens, block_table=block_table, out=out)
+    part, part_bytes = None, 0
+    if q.is_cuda:
+        part_bytes = lib.paged_attn_workspace(n, B, hq, hkv, hd, max_q, max_kv)
+        if part_bytes:
+            part = torch.empty(part_bytes // 4, dtype=torch.float32, device=q.device)
     lib.paged_attn(dev, stream, q.data_ptr(), q.stride(0), q.stride(1), pages.data_ptr(), pages.stride(0),
                    pages.stride(1), pages.stride(2), cu_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(),
                    block_table.stride(0), out.data_ptr(), out.stride(0), n, B, hq, hkv, hd, num, size, width,
-                   1.0 / math.sqrt(hd) if scale is None else float(scale), _ELEM[q.dtype])
+                   scale, _ELEM[q.dtype], max_q, max_kv,
+                   part.data_ptr() if part is not None else 0, part_bytes)
     return out
