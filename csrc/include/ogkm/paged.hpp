@@ -94,7 +94,7 @@ struct VerifyArgs {
   const int32_t* counts;     // [B] drafts of each request, or null: K
   int32_t* out;              // [B, K + 1], -1 behind the last token
   int32_t* accepted;         // [B]
-  double* sums;              // [B, nchunks, 2] partial sums (residual, target)
+  double* sums;              // [B, ceil(V / kVerifyChunk)] residual of each chunk
   uint32_t B, K, V, elem;
 };
 constexpr uint32_t kVerifyChunk = 4096;  // vocabulary entries of one partial sum

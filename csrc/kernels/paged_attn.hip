@@ -95,7 +95,8 @@ __device__ __forceinline__ bool nonfinite(u32x4 x) {
 // before that key, and special() adds what it does to the row's sum.
 constexpr int32_t kNever = INT32_MAX;
 template <typename T, int HD>
-__device__ __forceinline__ void take_special(u32x4& x, int32_t key, uint32_t dim, int32_t* first_key) {
+__device__ __forceinline__ void take_special(u32x4* v8, int32_t key, uint32_t dim, int32_t* first_key) {
+  u32x4 x = *v8;
   constexpr uint32_t inf = Mma<T>::kExp & 0xFFFFu;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -108,6 +109,7 @@ __device__ __forceinline__ void take_special(u32x4& x, int32_t key, uint32_t dim
         x[j] &= ~(0xFFFFu << s);
       }
     }
+  *v8 = x;
 }
 template <int HD>
 __device__ __forceinline__ float special(float o, int32_t pos, uint32_t dim, const int32_t* first_key) {
@@ -136,6 +138,16 @@ template <int HD>
 constexpr int kVRow = HD + 16;
 template <int HD>
 constexpr int kKVRow = kKRow<HD> + kVRow<HD>;  // elements of LDS per key
+
+// IEEE maximum: one v_maximum3_f32 takes three values (a NaN among them makes the
+// result NaN, which a NaN score makes of its row anyway), where fmaxf quiets
+// every operand first.
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float max_other_half(float x) {  // of lanes l and l ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t lo = r[0], hi = r[1];  // a bit_cast of r[1] itself would read r[0]
+  return max2(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
 
 // The wave's number, known to the compiler as uniform: bounds, page ids and
 // addresses that follow from it stay in scalar registers.
@@ -226,20 +238,26 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
     bool wave_special = false;
     // Page ids of this wave's next 32 blocks, one half block per lane (a page
     // holds at least 16 tokens), so that a block's addresses are wave-uniform.
+    const int32_t mine = (blocks - (int32_t)wave + kFewWaves - 1) / kFewWaves;
     int32_t ids = 0;
     auto fetch_ids = [&](int32_t n0) {
       const int32_t t = c0 + ((n0 + (int32_t)(lane >> 1)) * kFewWaves + (int32_t)wave) * 32 + 16 * (int32_t)(lane & 1);
       ids = t < c1 ? table[t >> a.page_shift] : 0;
     };
+    // The block ahead of the one multiplied, in registers. (Two were tried for 4
+    // column blocks, where a SIMD holds one wave: 150 registers spill and 32 x 5
+    // rows take 84 us, not 44.)
     u32x4 kr[2 * LD], vr[2 * LD];
-    bool miss0 = false, miss1 = false, next0 = false, next1 = false;
+    bool missing[2] = {};
     auto load = [&](int32_t n) {
+      if (n >= mine) return;
+      if ((n & 31) == 0) fetch_ids(n);
       const int32_t t0 = c0 + (n * kFewWaves + (int32_t)wave) * 32;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         int32_t page = __builtin_amdgcn_readlane(ids, 2 * (n & 31) + h);
         const bool miss = (uint32_t)page >= a.num_pages;
-        (h ? next1 : next0) = miss;
+        missing[h] = miss;
         if (miss) page = 0;
         const uint32_t row = (uint32_t)(t0 + 16 * h) & ((1u << a.page_shift) - 1u);
         const uint16_t* src = kbase + (uint64_t)page * a.page_stride + (uint64_t)row * HD;
@@ -250,40 +268,33 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
           vr[h * LD + j] = *reinterpret_cast<const u32x4*>(src + a.kv_stride + (j * 64 + lane) * 8);
       }
     };
-    const int32_t mine = (blocks - (int32_t)wave + kFewWaves - 1) / kFewWaves;
-    if (mine > 0) {
-      fetch_ids(0);
-      load(0);
-    }
+    load(0);
     for (int32_t n = 0; n < mine; ++n) {
+      const bool miss0 = missing[0], miss1 = missing[1];
       const int32_t t0 = c0 + (n * kFewWaves + (int32_t)wave) * 32;
-      miss0 = next0;
-      miss1 = next1;
       const bool masked = t0 + 31 > first;
       bool odd = false;
       if (masked) {
 #pragma unroll
         for (int j = 0; j < 2 * LD; ++j) odd |= nonfinite<T>(vr[j]);
-        if (__any(odd)) {
-          if (!wave_special)
-            for (uint32_t e = lane; e < 3 * HD; e += 64) first_key[wave][e] = kNever;
-          wave_special = true;
-          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int j = 0; j < 2 * LD; ++j)
-            take_special<T, HD>(vr[j], t0 + j * (512 / HD) + (int32_t)(lane / (HD / 8)), lane % (HD / 8) * 8, first_key[wave]);
-        }
       }
 #pragma unroll
       for (int j = 0; j < 2 * LD; ++j) {  // 512 / HD rows by each wave-wide store
         *reinterpret_cast<u32x4*>(kw + j * (512 / HD) * kKRow<HD>) = kr[j];
         *reinterpret_cast<u32x4*>(vw + j * (512 / HD) * kVRow<HD>) = vr[j];
       }
-      if (n + 1 < mine) {
-        if (((n + 1) & 31) == 0) fetch_ids(n + 1);
-        load(n + 1);
+      if (__any(odd)) {
+        if (!wave_special)
+          for (uint32_t e = lane; e < 3 * HD; e += 64) first_key[wave][e] = kNever;
+        wave_special = true;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int j = 0; j < 2 * LD; ++j)
+          take_special<T, HD>(reinterpret_cast<u32x4*>(vw + j * (512 / HD) * kVRow<HD>),
+                              t0 + j * (512 / HD) + (int32_t)(lane / (HD / 8)), lane % (HD / 8) * 8, first_key[wave]);
       }
+      load(n + 1);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       // S^T: two tiles of 16 keys
@@ -579,21 +590,22 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
     const int32_t t0 = c0 + i * kManyKeys;
     uint16_t* buf = lds + (i & 1) * kTile;
     const bool tile_masked = t0 + kManyKeys - 1 > first;
+    bool odd = false;
     if (tile_masked) {
-      bool odd = false;
 #pragma unroll
       for (int j = 0; j < LJ; ++j) odd |= nonfinite<T>(vr[j]);
-      if (odd) {
-        special_s = 1;
-#pragma unroll
-        for (int j = 0; j < LJ; ++j)
-          take_special<T, HD>(vr[j], t0 + j * (2048 / HD) + (int32_t)(tid / (HD / 8)), tid % (HD / 8) * 8, first_key);
-      }
     }
 #pragma unroll
     for (int j = 0; j < LJ; ++j) {
       *reinterpret_cast<u32x4*>(buf + kw + j * (2048 / HD) * kKRow<HD>) = kr[j];
       *reinterpret_cast<u32x4*>(buf + vw + j * (2048 / HD) * kVRow<HD>) = vr[j];
+    }
+    if (odd) {
+      special_s = 1;
+#pragma unroll 1
+      for (int j = 0; j < LJ; ++j)
+        take_special<T, HD>(reinterpret_cast<u32x4*>(buf + vw + j * (2048 / HD) * kVRow<HD>),
+                            t0 + j * (2048 / HD) + (int32_t)(tid / (HD / 8)), tid % (HD / 8) * 8, first_key);
     }
     miss = next_miss;
     if (i + 1 < tiles) load(i + 1);
@@ -610,6 +622,14 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
       for (int k = 0; k < KS; ++k)
         s[t] = Mma<T>::m32(*reinterpret_cast<const u32x4*>(buf + kread + t * 32 * kKRow<HD> + 16 * k), qf[k], s[t]);
     }
+    // six operands ahead of the products: an LDS read takes longer than one
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int k = 0; k < 2 * KS - 6; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     // register e of s[t] is key 32 t + 8 (e / 4) + 4 half + e % 4
     if (miss) {
 #pragma unroll
@@ -625,12 +645,12 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
         for (int e = 0; e < 16; ++e)
           if (t0 + 32 * t + 8 * (e / 4) + 4 * (int32_t)half + e % 4 > pos) s[t][e] = -__builtin_inff();
     }
-    float mx = fmaxf(s[0][0], s[1][0]);
+    float mx = max2(s[0][0], s[1][0]);
 #pragma unroll
-    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(s[0][e], s[1][e]));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+    for (int e = 1; e < 16; ++e) mx = max2(max2(mx, s[0][e]), s[1][e]);
+    mx = max_other_half(mx) * c;
     if (__any(mx > m + kLazy) || i == 0) {
-      const float mn = fmaxf(m, mx);
+      const float mn = max2(m, mx);
       const float f = m == mn ? 1.f : m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
       l *= f;
 #pragma unroll
@@ -638,25 +658,50 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
       m = mn;
     }
     const float base = (m == -__builtin_inff() ? 0.f : m) - kShift<T>;
-    u32x4 p[4];  // B operands of the four groups of 16 keys
+    // Probabilities of keys 16 kt .. (registers 8 (kt % 2) .. of s[kt / 2]) as a B operand
+    auto exponentials = [&](int kt) {
+      u32x4 p;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -base)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], c, -base));
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt / 2][8 * (kt % 2) + 2 * e], c, -base));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt / 2][8 * (kt % 2) + 2 * e + 1], c, -base));
         l += p0 + p1;
-        p[2 * t + e / 8][(e % 8) / 2] = pack2<T>(p0, p1);
+        p[e] = pack2<T>(p0, p1);
       }
+      return p;
+    };
     // V^T operand of dims 32 d .., keys 16 kt ..: two 16-dim halves by lane group
     auto v_frag = [&](int d, int kt) {
       const uint16_t* at = buf + vread + 16 * kt * kVRow<HD> + 32 * d;
       const u32x2 lo = read_tr(at), hi = read_tr(at + 8 * kVRow<HD>);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
+    // The products of one group of 16 keys run beside the exponentials and the
+    // operand reads of the next.
+    u32x4 va[2][DT], p[2];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+    for (int d = 0; d < DT; ++d) va[0][d] = v_frag(d, 0);
+    p[0] = exponentials(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] = Mma<T>::m32(v_frag(d, kt), p[kt], o[d]);
+    for (int kt = 0; kt < 4; ++kt) {
+      if (kt < 3) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) va[(kt + 1) & 1][d] = v_frag(d, kt + 1);
+        p[(kt + 1) & 1] = exponentials(kt + 1);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] = Mma<T>::m32(va[kt & 1][d], p[kt & 1], o[d]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        __builtin_amdgcn_sched_group_barrier(0x002, 10 / DT, 1);
+        __builtin_amdgcn_sched_group_barrier(0x400, 8 / DT, 1);
+        __builtin_amdgcn_sched_group_barrier(0x002, 10 / DT, 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
   l += __shfl_xor(l, 32, 64);
   if (!in) return;
@@ -757,17 +802,42 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttnArgs a) {
   if (rq.kv > rq.cap) return;
   const int32_t used = splits_used(keys, split_keys(keys, splits));
   if (used == 1) return;
-  float big = -__builtin_inff();
-  for (int32_t s = 0; s < used; ++s) big = fmaxf(big, a.part_ml[2 * (at + (uint64_t)s * R)]);
-  float sum = 0.f, o[E] = {};
-#pragma unroll 4
-  for (int32_t s = 0; s < used; ++s) {
-    const uint64_t i = at + (uint64_t)s * R;
-    const float m = a.part_ml[2 * i];
-    const float f = m == -__builtin_inff() ? (big == m ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - big);
-    sum += f * a.part_ml[2 * i + 1];
+  // lane: split s0 + lane. Its weight is broadcast while the wave adds the splits'
+  // rows, eight loads in flight.
+  float big = -__builtin_inff(), sum = 0.f, o[E] = {};
+  for (int32_t s0 = 0; s0 < used; s0 += 64) {
+    const int32_t left = min(used - s0, 64);
+    const bool on = (int32_t)lane < left;
+    const uint64_t i = at + (uint64_t)(s0 + (on ? (int32_t)lane : 0)) * R;
+    const float m = on ? a.part_ml[2 * i] : -__builtin_inff(), l = on ? a.part_ml[2 * i + 1] : 0.f;
+    float mx = m;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += f * a.part_o[i * HD + lane * E + e];
+    for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+    mx = fmaxf(mx, big);
+    const float old = big == mx ? 1.f : big == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(big - mx);
+    const float f = m == mx ? 1.f : m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+    float ls = on ? f * l : 0.f;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) ls += __shfl_xor(ls, d, 64);
+    sum = sum * old + ls;
+    big = mx;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= old;
+    const float* po = a.part_o + (at + (uint64_t)s0 * R) * HD + lane * E;
+    for (int32_t s = 0; s < left; s += 8) {
+      float x[8][E];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = po[(uint64_t)min(s + u, left - 1) * R * HD + e];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s + u, left - 1)));
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (s + u < left) o[e] += w * x[u][e];
+      }
+    }
   }
   const uint32_t tok = (uint32_t)r / g, h = (uint32_t)r - tok * g;
   const bool none = rq.kv - rq.n + (int32_t)tok < 0;
@@ -820,10 +890,17 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
     p.few_rows = g <= 64 ? 16 * p.few_blocks : 0;
     p.many_tiles = (uint32_t)(n * g / kManyRows + std::min<uint64_t>(B, n * g / (p.few_rows + 1)));
     const uint64_t wgs = std::max<uint64_t>(p.many_tiles * heads, 1);
+    // two workgroups a CU; more splits only add partial results (48 mixed
+    // requests of 64-wide heads: 55 us at 512, 91 at 1024)
     p.many_splits = (uint32_t)std::min<uint64_t>((512 + wgs - 1) / wgs, key_splits);
   }
   const uint64_t wgs = std::max<uint64_t>(B * heads, 1);
-  p.few_splits = (uint32_t)std::min<uint64_t>((1024 + wgs - 1) / wgs, key_splits);
+  // A workgroup a CU: four waves with a block each in flight draw what HBM gives.
+  // us at 128 / 256 / 512 / 1024 workgroups: 4 requests of up to 131071 keys 343 /
+  // 257 / 257 / 257, 16 of 4096 49 / 42 / 44 / 44, 64 of 2048 (70B heads) 70 / 70 /
+  // 70 / 78, 32 x 5 rows of 8191 (one kv head) 126 / 44 / 58 / 82. At least kMinSplit keys
+  // each: 128, 256 and 512 are within 2 us, 1024 loses 3 on 4 requests of 8192.
+  p.few_splits = (uint32_t)std::min<uint64_t>((256 + wgs - 1) / wgs, key_splits);
   p.few_part = p.few_splits > 1 ? wgs * p.few_splits * 16 * p.few_blocks : 0;
   p.part_rows = p.few_part + (p.many_splits > 1 ? p.many_tiles * heads * p.many_splits * kManyRows : 0);
   return p;

@@ -42,6 +42,15 @@ Runtime* rt() {
   return r;
 }
 
+// The tensors of a call are on the kind of device the backend runs on (dev < 0:
+// host memory). A kernel must never see host memory, nor the fake backend a GPU's.
+int device_of(int dev, const char* what) {
+  if (rt()->be()->is_fake() != (dev < 0))
+    throw py::value_error(std::string(what) + (dev < 0 ? ": tensors must be on a GPU"
+                                                       : ": the fake backend takes CPU tensors"));
+  return std::max(dev, 0);
+}
+
 // log2 of a page size the paged kernels take: a power of two of 16 .. 256 tokens.
 uint32_t page_shift_of(uint32_t page_size, const char* what) {
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
@@ -1130,25 +1139,25 @@ PYBIND11_MODULE(_ogkm, m) {
      py::arg("scale"), py::arg("out_frag") = false, py::arg("split_tokens") = 0);
   // Paged serving and speculative decoding (ops/paged.py, ops/speculative.py).
   m.def("paged_plan_max_requests", [] { return kPlanMaxRequests; });
+  // `out`: cu_q [B + 1], kv_lens [B], page_counts [B], granted [B], positions and
+  // slots [n_tokens], free_start [1], one behind the other.
   m.def("paged_plan", [](int dev, uint64_t stream, uint64_t new_lens, uint64_t kv_lens, uint64_t page_counts,
-                         uint64_t table, uint64_t table_ld, uint64_t free_pages, uint64_t free_start, uint64_t cu_q,
-                         uint64_t kv_out, uint64_t counts_out, uint64_t granted, uint64_t positions, uint64_t slots,
-                         uint64_t free_out, uint32_t B, uint32_t width, uint32_t n_free, uint32_t page_size,
-                         uint32_t n_tokens) {
+                         uint64_t table, uint64_t table_ld, uint64_t free_pages, uint64_t free_start, uint64_t out,
+                         uint32_t B, uint32_t width, uint32_t n_free, uint32_t page_size, uint32_t n_tokens) {
     const uint32_t shift = page_shift_of(page_size, "paged_plan");
     if (B > kPlanMaxRequests) throw StatusError("paged_plan: too many requests");
     if ((uint64_t)width * page_size > INT32_MAX || n_free > INT32_MAX || n_tokens > INT32_MAX)
       throw StatusError("paged_plan: positions, free pages and rows are 32-bit");
+    int32_t* o = (int32_t*)out;
+    int32_t* rows = o + 4 * (uint64_t)B + 1;
     PlanArgs a{(const int32_t*)new_lens, (const int32_t*)kv_lens, (const int32_t*)page_counts, (int32_t*)table,
-               (const int32_t*)free_pages, (const int32_t*)free_start, (int32_t*)cu_q, (int32_t*)kv_out,
-               (int32_t*)counts_out, (int32_t*)granted, (int32_t*)positions, (int32_t*)slots, (int32_t*)free_out,
-               table_ld, B, width, n_free, shift, n_tokens};
-    check(rt()->be()->paged_plan(dev, a, (void*)stream), "paged_plan");
+               (const int32_t*)free_pages, (const int32_t*)free_start, o, o + B + 1, o + 2 * (uint64_t)B + 1,
+               o + 3 * (uint64_t)B + 1, rows, rows + n_tokens, rows + 2 * (uint64_t)n_tokens, table_ld, B, width,
+               n_free, shift, n_tokens};
+    check(rt()->be()->paged_plan(device_of(dev, "paged_plan"), a, (void*)stream), "paged_plan");
   }, py::arg("dev"), py::arg("stream"), py::arg("new_lens"), py::arg("kv_lens"), py::arg("page_counts"),
-     py::arg("table"), py::arg("table_ld"), py::arg("free_pages"), py::arg("free_start"), py::arg("cu_q"),
-     py::arg("kv_out"), py::arg("counts_out"), py::arg("granted"), py::arg("positions"), py::arg("slots"),
-     py::arg("free_out"), py::arg("B"), py::arg("width"), py::arg("n_free"), py::arg("page_size"),
-     py::arg("n_tokens"));
+     py::arg("table"), py::arg("table_ld"), py::arg("free_pages"), py::arg("free_start"), py::arg("out"),
+     py::arg("B"), py::arg("width"), py::arg("n_free"), py::arg("page_size"), py::arg("n_tokens"));
   m.def("paged_rope", [](int dev, uint64_t stream, uint64_t qkv, uint64_t ldqkv, uint64_t cos, uint64_t sin,
                          uint64_t positions, uint64_t slots, uint64_t q_out, uint64_t pages, uint64_t kv_stride,
                          uint64_t page_stride, uint64_t head_stride, uint32_t n, uint32_t hq, uint32_t hkv, uint32_t hd,
@@ -1159,7 +1168,7 @@ PYBIND11_MODULE(_ogkm, m) {
     PagedRopeArgs a{(const uint16_t*)qkv, ldqkv, (const float*)cos, (const float*)sin, (const int32_t*)positions,
                     (const int32_t*)slots, (uint16_t*)q_out, (uint16_t*)pages, kv_stride, page_stride, head_stride,
                     n, hq, hkv, hd, num_pages, shift, max_pos, elem};
-    check(rt()->be()->paged_rope(dev, a, (void*)stream), "paged_rope");
+    check(rt()->be()->paged_rope(device_of(dev, "paged_rope"), a, (void*)stream), "paged_rope");
   }, py::arg("dev"), py::arg("stream"), py::arg("qkv"), py::arg("ldqkv"), py::arg("cos"), py::arg("sin"),
      py::arg("positions"), py::arg("slots"), py::arg("q_out"), py::arg("pages"), py::arg("kv_stride"),
      py::arg("page_stride"), py::arg("head_stride"), py::arg("n"), py::arg("hq"), py::arg("hkv"), py::arg("hd"),
@@ -1182,7 +1191,7 @@ PYBIND11_MODULE(_ogkm, m) {
     if (!rt()->be()->is_fake() && a.plan.part_rows * (hd + 2) * 4 > part_bytes) throw StatusError("paged_attn: partial workspace too small");
     a.part_o = (float*)part;
     a.part_ml = (float*)part + a.plan.part_rows * hd;
-    check(rt()->be()->paged_attn(dev, a, (void*)stream), "paged_attn");
+    check(rt()->be()->paged_attn(device_of(dev, "paged_attn"), a, (void*)stream), "paged_attn");
   }, py::arg("dev"), py::arg("stream"), py::arg("q"), py::arg("q_stride"), py::arg("q_head_stride"),
      py::arg("pages"), py::arg("kv_stride"), py::arg("page_stride"), py::arg("head_stride"), py::arg("cu_q"),
      py::arg("kv_lens"), py::arg("table"), py::arg("table_ld"), py::arg("out"), py::arg("out_stride"), py::arg("n"),
@@ -1194,22 +1203,20 @@ PYBIND11_MODULE(_ogkm, m) {
     return hkv ? paged_attn_plan(n, B, hq, hkv, hd, max_q, max_kv).part_rows * (hd + 2) * 4 : 0;
   }, py::arg("n"), py::arg("B"), py::arg("hq"), py::arg("hkv"), py::arg("hd"), py::arg("max_q"), py::arg("max_kv"));
   m.def("verify_chunk", [] { return kVerifyChunk; });
+  // `sums`: ceil(V / verify_chunk()) doubles a request.
   m.def("verify_draft", [](int dev, uint64_t stream, uint64_t p, uint64_t p_batch, uint64_t p_row, uint64_t q,
                            uint64_t q_batch, uint64_t q_row, uint64_t tokens, uint64_t u, uint64_t u_last,
-                           uint64_t counts, uint64_t out, uint64_t accepted, uint64_t sums, uint64_t sums_bytes,
-                           uint32_t B, uint32_t K, uint32_t V, uint32_t elem) {
-    if (!V || V > INT32_MAX || K > 65535 || B > 65535 || elem > ELEM_F32)
-      throw StatusError("verify_draft: 1 <= V < 2^31, B and K <= 65535, bf16, fp16 or f32");
-    if ((uint64_t)B * ((V + kVerifyChunk - 1) / kVerifyChunk) * 16 > sums_bytes)
-      throw StatusError("verify_draft: workspace too small");
+                           uint64_t counts, uint64_t out, uint64_t accepted, uint64_t sums, uint32_t B,
+                           uint32_t K, uint32_t V, uint32_t elem) {
+    if (!V || V > (1u << 30) || K > 65535 || B > 65535 || elem > ELEM_F32)
+      throw StatusError("verify_draft: 1 <= V <= 2^30, B and K <= 65535, bf16, fp16 or f32");
     VerifyArgs a{(const void*)p, p_batch, p_row, (const void*)q, q_batch, q_row, (const int32_t*)tokens,
                  (const float*)u, (const float*)u_last, (const int32_t*)counts, (int32_t*)out, (int32_t*)accepted,
                  (double*)sums, B, K, V, elem};
-    check(rt()->be()->verify_draft(dev, a, (void*)stream), "verify_draft");
+    check(rt()->be()->verify_draft(device_of(dev, "verify_draft"), a, (void*)stream), "verify_draft");
   }, py::arg("dev"), py::arg("stream"), py::arg("p"), py::arg("p_batch"), py::arg("p_row"), py::arg("q"),
      py::arg("q_batch"), py::arg("q_row"), py::arg("tokens"), py::arg("u"), py::arg("u_last"), py::arg("counts"),
-     py::arg("out"), py::arg("accepted"), py::arg("sums"), py::arg("sums_bytes"), py::arg("B"), py::arg("K"),
-     py::arg("V"), py::arg("elem"));
+     py::arg("out"), py::arg("accepted"), py::arg("sums"), py::arg("B"), py::arg("K"), py::arg("V"), py::arg("elem"));
   m.def("fault_buffer_info", [](int dev) {
     DeviceFaultBuffer& fb = rt()->dev(dev).fault_buf;
     py::dict d;

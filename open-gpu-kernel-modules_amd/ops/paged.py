@@ -21,64 +21,76 @@ share none.
 """
 from __future__ import annotations
 
-import math
-from dataclasses import dataclass
+import functools
+from typing import NamedTuple
 
 import torch
 
 from .._native import lib
 
 _ELEM = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_I32 = torch.int32
+
+# The checks of shapes, strides and types of a call run once per layout: a decode
+# step calls these ops with the same layouts over and over, and on the smallest
+# ones the host is what limits the rate. Nothing of a tensor's content, address
+# or identity is kept.
+_per_layout = functools.lru_cache(maxsize=512)
 
 
-def _where(op: str, first: torch.Tensor, **tensors: torch.Tensor) -> tuple[int, int]:
-    """(device index, stream) of a call. Every tensor has to be on the first
-    one's device, and that has to be the runtime backend's kind of device."""
-    for name, t in tensors.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{op}: {name} is on {t.device}, expected {first.device}")
-    if lib.backend_name() == "fake":
-        if first.device.type != "cpu":
-            raise ValueError(f"{op}: the fake backend takes CPU tensors")
-        return 0, 0
-    if first.device.type != "cuda":
+def _where(op: str, first: torch.Tensor, *others: torch.Tensor) -> tuple[int, int]:
+    """(device index, stream) of a call, (-1, 0) on the host. Every tensor has to be
+    on the first one's device; the binding checks that the backend runs there."""
+    if first.is_cuda:
+        dev = first.get_device()
+        for t in others:
+            if t.get_device() != dev:
+                raise ValueError(f"{op}: tensors on {first.device} and {t.device}")
+        return dev, torch._C._cuda_getCurrentRawStream(dev)
+    for t in others:
+        if t.device != first.device:
+            raise ValueError(f"{op}: tensors on {first.device} and {t.device}")
+    if first.device.type != "cpu":
         raise ValueError(f"{op}: tensors must be on a GPU")
-    dev = first.device.index
-    return dev, int(torch.cuda.current_stream(dev).cuda_stream)
+    return -1, 0
 
 
 def _ints(op: str, name: str, t: torch.Tensor, shape: tuple) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{op}: {name} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
-def _table(op: str, table: torch.Tensor, B: int) -> None:
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or (
-            table.shape[1] > 1 and table.stride(1) != 1) or (B > 1 and table.stride(0) < table.shape[1]):
+def _check_table(op: str, dtype, shape, stride, B: int) -> None:
+    if dtype is not _I32 or len(shape) != 2 or shape[0] != B or shape[1] < 1 or (
+            shape[1] > 1 and stride[1] != 1) or (B > 1 and stride[0] < shape[1]):
         raise ValueError(f"{op}: block_table must be int32 [{B}, width] with rows apart")
 
 
-def _page_size(op: str, size: int) -> None:
+def _check_page_size(op: str, size: int) -> None:
     if size < 16 or size > 256 or size & (size - 1):
         raise ValueError(f"{op}: page size must be a power of two of 16 .. 256 tokens, got {size}")
 
 
-def _pool(op: str, pages: torch.Tensor, like: torch.Tensor | None = None) -> None:
-    if pages.dim() != 5 or pages.shape[0] != 2 or pages.dtype not in (torch.bfloat16, torch.float16):
+def _check_pool(op: str, dtype, shape, stride, rows_dtype) -> None:
+    if len(shape) != 5 or shape[0] != 2 or dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"{op}: pages must be bf16 or fp16 [2, num_pages, hkv, page_size, hd]")
-    _, num, hkv, size, hd = pages.shape
-    _page_size(op, size)
-    if num * size > 2**31 - 1 or num < 1 or hkv < 1:
-        raise ValueError(f"{op}: the pool must hold 1 .. 2^31 - 1 slots of at least one head")
-    if pages.stride(4) != 1 or pages.stride(3) != hd or any(
-            n > 1 and (st % 8 or st < 0) for n, st in zip(pages.shape[:3], pages.stride()[:3])) or pages.data_ptr() % 16:
+    _, num, hkv, size, hd = shape
+    _check_page_size(op, size)
+    if num * size > 2**31 - 1 or num < 1 or hkv < 1 or hkv > 65535:
+        raise ValueError(f"{op}: the pool must hold 1 .. 2^31 - 1 slots of 1 .. 65535 heads")
+    if stride[4] != 1 or stride[3] != hd or any(n > 1 and st % 8 for n, st in zip(shape[:3], stride[:3])):
         raise ValueError(f"{op}: a page's rows must be contiguous and 16-byte aligned")
-    if like is not None and like.dtype != pages.dtype:
-        raise ValueError(f"{op}: {like.dtype} rows over {pages.dtype} pages")
+    if rows_dtype != dtype:
+        raise ValueError(f"{op}: {rows_dtype} rows over {dtype} pages")
 
 
-@dataclass
-class Plan:
+def _aligned(op: str, *pointers: int) -> None:
+    for p in pointers:
+        if p % 16:
+            raise ValueError(f"{op}: tensors must be 16-byte aligned")
+
+
+class Plan(NamedTuple):
     """One step of a batch, all int32 on the device. ``granted[b]`` is 0 where
     request b's pages did not fit the free list or its table row, or its rows
     did not fit n_tokens: its lengths and pages then stay as they were and its
@@ -102,30 +114,33 @@ def plan(new_lens: torch.Tensor, kv_lens: torch.Tensor, page_counts: torch.Tenso
     the ``page_counts[b]`` it holds - a count of its own, since a request whose
     drafts were refused keeps pages beyond its length. One launch; at most
     4096 requests. Negative lengths and counts are taken as 0."""
-    B = new_lens.shape[0] if new_lens.dim() == 1 else -1
-    for name, t in (("new_lens", new_lens), ("kv_lens", kv_lens), ("page_counts", page_counts)):
-        _ints("plan", name, t, (B,))
-    _table("plan", block_table, B)
-    _page_size("plan", page_size)
-    if free_pages.dim() != 1:
-        raise ValueError("plan: free_pages must be a list of pages")
-    _ints("plan", "free_pages", free_pages, (free_pages.shape[0],))
+    B, n_free = _plan_layout(new_lens.shape, block_table.dtype, block_table.shape, block_table.stride(),
+                             free_pages.shape, page_size, n_tokens)
+    shape = (B,)
+    _ints("plan", "new_lens", new_lens, shape)
+    _ints("plan", "kv_lens", kv_lens, shape)
+    _ints("plan", "page_counts", page_counts, shape)
+    _ints("plan", "free_pages", free_pages, (n_free,))
     _ints("plan", "free_start", free_start, (1,))
-    width = block_table.shape[1]
-    if B > lib.paged_plan_max_requests() or not 0 <= n_tokens < 2**31 or width * page_size >= 2**31 \
-            or free_pages.shape[0] >= 2**31:
-        raise ValueError(f"plan: at most {lib.paged_plan_max_requests()} requests; rows and positions below 2^31")
-    dev, stream = _where("plan", new_lens, kv_lens=kv_lens, page_counts=page_counts, block_table=block_table,
-                         free_pages=free_pages, free_start=free_start)
+    dev, stream = _where("plan", new_lens, kv_lens, page_counts, block_table, free_pages, free_start)
     # one allocation for the seven outputs
-    sizes = (B + 1, B, B, B, n_tokens, n_tokens, 1)
-    parts = torch.empty(sum(sizes), dtype=torch.int32, device=new_lens.device).split(sizes)
-    cu, kv, counts, granted, positions, slots, start = parts
+    out = new_lens.new_empty(4 * B + 2 * n_tokens + 2)
     lib.paged_plan(dev, stream, new_lens.data_ptr(), kv_lens.data_ptr(), page_counts.data_ptr(),
                    block_table.data_ptr(), block_table.stride(0), free_pages.data_ptr(), free_start.data_ptr(),
-                   cu.data_ptr(), kv.data_ptr(), counts.data_ptr(), granted.data_ptr(), positions.data_ptr(),
-                   slots.data_ptr(), start.data_ptr(), B, width, free_pages.shape[0], page_size, n_tokens)
-    return Plan(cu, kv, counts, granted, positions, slots, start)
+                   out.data_ptr(), B, block_table.shape[1], n_free, page_size, n_tokens)
+    return Plan(*out.split_with_sizes((B + 1, B, B, B, n_tokens, n_tokens, 1)))
+
+
+@_per_layout
+def _plan_layout(lens, table_dtype, table, table_stride, free, page_size, n_tokens):
+    if len(lens) != 1 or len(free) != 1:
+        raise ValueError("plan: lengths and free_pages must be lists")
+    B, most = lens[0], lib.paged_plan_max_requests()
+    _check_table("plan", table_dtype, table, table_stride, B)
+    _check_page_size("plan", page_size)
+    if B > most or not 0 <= n_tokens < 2**31 or table[1] * page_size >= 2**31 or free[0] >= 2**31:
+        raise ValueError(f"plan: at most {most} requests; rows and positions below 2^31")
+    return B, free[0]
 
 
 def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor,
@@ -136,26 +151,36 @@ def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pages: torc
     nothing is stored, as for a slot outside the pool; a position behind the
     tables gives NaN. Slots of one call are distinct (of two rows with one slot
     either's values may stay)."""
-    _pool("rope_kv", pages, qkv)
-    _, num, heads, size, hd = pages.shape
+    n, hd, num, size, max_pos = _rope_layout(qkv.dtype, qkv.shape, qkv.stride(), pages.dtype, pages.shape,
+                                             pages.stride(), cos.dtype, cos.shape, cos.stride(), sin.dtype, sin.shape,
+                                             sin.stride(), hq, hkv)
+    shape = (n,)
+    _ints("rope_kv", "positions", positions, shape)
+    _ints("rope_kv", "slots", slots, shape)
+    dev, stream = _where("rope_kv", qkv, cos, sin, pages, positions, slots)
+    q = qkv.new_empty((n, hq, hd))
+    x, c, s, p = qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), pages.data_ptr()
+    _aligned("rope_kv", x, c, s, p)
+    kv_stride, page_stride, head_stride = pages.stride()[:3]
+    lib.paged_rope(dev, stream, x, qkv.stride(0), c, s, positions.data_ptr(), slots.data_ptr(), q.data_ptr(), p,
+                   kv_stride, page_stride, head_stride, n, hq, hkv, hd, num, size, max_pos, _ELEM[qkv.dtype])
+    return q
+
+
+@_per_layout
+def _rope_layout(dtype, qkv, qkv_stride, pool_dtype, pool, pool_stride, cos_dtype, cos, cos_stride, sin_dtype, sin,
+                 sin_stride, hq, hkv):
+    _check_pool("rope_kv", pool_dtype, pool, pool_stride, dtype)
+    _, num, heads, size, hd = pool
     if hkv != heads or hq < 1 or hd % 16:
         raise ValueError(f"rope_kv: {hkv} kv heads over a pool of {heads}, hd {hd} (a multiple of 16)")
-    if qkv.dim() != 2 or qkv.shape[1] != (hq + 2 * hkv) * hd or qkv.stride(1) != 1 or (
-            qkv.shape[0] > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < 0)) or qkv.data_ptr() % 16:
+    if len(qkv) != 2 or qkv[1] != (hq + 2 * hkv) * hd or qkv_stride[1] != 1 or (qkv[0] > 1 and qkv_stride[0] % 8):
         raise ValueError("rope_kv: qkv must be [n, (hq + 2 hkv) hd] with contiguous, 16-byte aligned rows")
-    n = qkv.shape[0]
-    _ints("rope_kv", "positions", positions, (n,))
-    _ints("rope_kv", "slots", slots, (n,))
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] * 2 != hd or not t.is_contiguous() \
-                or t.shape != cos.shape or t.shape[0] < 1 or t.shape[0] >= 2**31 or t.data_ptr() % 16:
+    for name, d, shape, stride in (("cos", cos_dtype, cos, cos_stride), ("sin", sin_dtype, sin, sin_stride)):
+        if d is not torch.float32 or len(shape) != 2 or shape[1] * 2 != hd or stride != (hd // 2, 1) \
+                or shape != cos or not 1 <= shape[0] < 2**31:
             raise ValueError(f"rope_kv: {name} must be contiguous f32 [max_pos, {hd // 2}]")
-    dev, stream = _where("rope_kv", qkv, cos=cos, sin=sin, pages=pages, positions=positions, slots=slots)
-    q = torch.empty(n, hq, hd, dtype=qkv.dtype, device=qkv.device)
-    lib.paged_rope(dev, stream, qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
-                   slots.data_ptr(), q.data_ptr(), pages.data_ptr(), pages.stride(0), pages.stride(1), pages.stride(2),
-                   n, hq, hkv, hd, num, size, cos.shape[0], _ELEM[qkv.dtype])
-    return q
+    return qkv[0], hd, num, size, cos[0]
 
 
 def attention(q: torch.Tensor, pages: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor,
@@ -170,42 +195,51 @@ def attention(q: torch.Tensor, pages: torch.Tensor, cu_q: torch.Tensor, kv_lens:
 
     ``max_q`` / ``max_kv``: the host's bounds of rows and length per request; they
     only choose how the work is split (default: n and the table's width)."""
-    _pool("attention", pages, q)
-    _, num, hkv, size, hd = pages.shape
-    if hd not in (64, 128):
-        raise ValueError(f"attention: head dim 64 or 128, got {hd}")
-    if q.dim() != 3 or q.shape[2] != hd or q.shape[1] < 1 or q.shape[1] % hkv:
-        raise ValueError(f"attention: q must be [n, hq, {hd}] with hq a multiple of {hkv}")
-    n, hq = q.shape[:2]
-    if q.stride(2) != 1 or any(c > 1 and (s % 8 or s < 0) for c, s in zip(q.shape[:2], q.stride()[:2])) \
-            or q.data_ptr() % 16 or n >= 2**31:
-        raise ValueError("attention: q's heads must be contiguous and 16-byte aligned")
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+    n, B, hq, hkv, hd, num, size, width = _attention_layout(
+        q.dtype, q.shape, q.stride(), pages.dtype, pages.shape, pages.stride(), kv_lens.shape, block_table.dtype,
+        block_table.shape, block_table.stride())
     _ints("attention", "kv_lens", kv_lens, (B,))
     _ints("attention", "cu_q", cu_q, (B + 1,))
-    _table("attention", block_table, B)
-    width = block_table.shape[1]
-    if width * size > 2**30 or B > 65535 or hkv > 65535:
-        raise ValueError("attention: at most 2^30 tokens per request, 65535 requests and kv heads")
     max_q = n if max_q is None else min(max(int(max_q), 1), n)
     max_kv = width * size if max_kv is None else min(max(int(max_kv), 1), width * size)
     if out is None:
-        out = torch.empty(n, hq * hd, dtype=q.dtype, device=q.device)
+        out = q.new_empty((n, hq * hd))
     elif out.dtype != q.dtype or tuple(out.shape) != (n, hq * hd) or out.stride(1) != 1 or (
-            n > 1 and (out.stride(0) % 8 or out.stride(0) < hq * hd)) or out.data_ptr() % 16:
+            n > 1 and (out.stride(0) % 8 or out.stride(0) < hq * hd)):
         raise ValueError(f"attention: out must be {q.dtype} [{n}, {hq * hd}] with contiguous, aligned rows")
-    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    scale = hd ** -0.5 if scale is None else float(scale)
     if not 1e-30 < abs(scale) < 1e30:
         raise ValueError(f"attention: scale {scale}")
-    dev, stream = _where("attention", q, pages=pages, cu_q=cu_q, kv_lens=kv_lens, block_table=block_table, out=out)
-    part, part_bytes = None, 0
-    if q.is_cuda:
+    dev, stream = _where("attention", q, pages, cu_q, kv_lens, block_table, out)
+    part, part_bytes = 0, 0
+    if dev >= 0:
         part_bytes = lib.paged_attn_workspace(n, B, hq, hkv, hd, max_q, max_kv)
         if part_bytes:
-            part = torch.empty(part_bytes // 4, dtype=torch.float32, device=q.device)
-    lib.paged_attn(dev, stream, q.data_ptr(), q.stride(0), q.stride(1), pages.data_ptr(), pages.stride(0),
-                   pages.stride(1), pages.stride(2), cu_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(),
-                   block_table.stride(0), out.data_ptr(), out.stride(0), n, B, hq, hkv, hd, num, size, width,
-                   scale, _ELEM[q.dtype], max_q, max_kv,
-                   part.data_ptr() if part is not None else 0, part_bytes)
+            work = torch.empty(part_bytes, dtype=torch.uint8, device=q.device)
+            part = work.data_ptr()
+    x, p, y = q.data_ptr(), pages.data_ptr(), out.data_ptr()
+    _aligned("attention", x, p, y)
+    q_stride, q_head_stride, _ = q.stride()
+    kv_stride, page_stride, head_stride = pages.stride()[:3]
+    lib.paged_attn(dev, stream, x, q_stride, q_head_stride, p, kv_stride, page_stride, head_stride, cu_q.data_ptr(),
+                   kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), y, out.stride(0), n, B, hq, hkv,
+                   hd, num, size, width, scale, _ELEM[q.dtype], max_q, max_kv, part, part_bytes)
     return out
+
+
+@_per_layout
+def _attention_layout(dtype, q, q_stride, pool_dtype, pool, pool_stride, lens, table_dtype, table, table_stride):
+    _check_pool("attention", pool_dtype, pool, pool_stride, dtype)
+    _, num, hkv, size, hd = pool
+    if hd not in (64, 128):
+        raise ValueError(f"attention: head dim 64 or 128, got {hd}")
+    if len(q) != 3 or q[2] != hd or q[1] < 1 or q[1] % hkv:
+        raise ValueError(f"attention: q must be [n, hq, {hd}] with hq a multiple of {hkv}")
+    if q_stride[2] != 1 or any(c > 1 and s % 8 for c, s in zip(q[:2], q_stride[:2])) or q[0] >= 2**31:
+        raise ValueError("attention: q's heads must be contiguous and 16-byte aligned")
+    if len(lens) != 1 or lens[0] > 65535:
+        raise ValueError("attention: kv_lens must list at most 65535 requests")
+    _check_table("attention", table_dtype, table, table_stride, lens[0])
+    if table[1] * size > 2**30:
+        raise ValueError("attention: at most 2^30 tokens per request")
+    return q[0], lens[0], q[1], hkv, hd, num, size, table[1]

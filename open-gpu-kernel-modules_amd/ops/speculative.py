@@ -12,13 +12,23 @@ from __future__ import annotations
 import torch
 
 from .._native import lib
-from .paged import _ELEM, _ints, _where
+from .paged import _ELEM, _ints, _per_layout, _where
 
 
-def _rows(name: str, t: torch.Tensor, shape: tuple) -> None:
-    if t.dim() != 3 or tuple(t.shape) != shape or t.dtype not in _ELEM or (t.shape[2] > 1 and t.stride(2) != 1) \
-            or any(n > 1 and s < 0 for n, s in zip(t.shape, t.stride())):
-        raise ValueError(f"verify_draft: {name} must be f32, bf16 or fp16 {list(shape)} with contiguous rows")
+@_per_layout
+def _layout(dtype, shape, stride, q_dtype, q_shape, q_stride):
+    if len(shape) != 3 or shape[1] < 1 or not 1 <= shape[2] <= 2**30:
+        raise ValueError("verify_draft: target_probs must be [B, K + 1, V]")
+    B, K, V = shape[0], shape[1] - 1, shape[2]
+    if B > 65535 or K > 65535:
+        raise ValueError("verify_draft: at most 65535 requests and drafts")
+    for name, d, got, st, want in (("target_probs", dtype, shape, stride, (B, K + 1, V)),
+                                   ("draft_probs", q_dtype, q_shape, q_stride, (B, K, V))):
+        if d is not None and (got != want or d not in _ELEM or (V > 1 and st[2] != 1)):
+            raise ValueError(f"verify_draft: {name} must be f32, bf16 or fp16 {list(want)} with contiguous rows")
+    if q_dtype not in (None, dtype):
+        raise ValueError(f"verify_draft: {q_dtype} drafts against a {dtype} target")
+    return B, K, V, -(-V // lib.verify_chunk())
 
 
 def verify_draft(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, draft_tokens: torch.Tensor,
@@ -36,32 +46,28 @@ def verify_draft(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, d
     nothing remains), then -1. Rows need not be normalised. A token outside the
     vocabulary is refused; a NaN or negative probability weighs nothing; a row
     without any weight gives -1."""
-    if target_probs.dim() != 3 or target_probs.shape[1] < 1 or not 1 <= target_probs.shape[2] < 2**31:
-        raise ValueError("verify_draft: target_probs must be [B, K + 1, V]")
-    B, K, V = target_probs.shape[0], target_probs.shape[1] - 1, target_probs.shape[2]
-    if B > 65535 or K > 65535:
-        raise ValueError("verify_draft: at most 65535 requests and drafts")
-    _rows("target_probs", target_probs, (B, K + 1, V))
-    if draft_probs is not None:
-        _rows("draft_probs", draft_probs, (B, K, V))
-        if draft_probs.dtype != target_probs.dtype:
-            raise ValueError(f"verify_draft: {draft_probs.dtype} drafts against a {target_probs.dtype} target")
+    p, q = target_probs, draft_probs
+    if q is None:
+        B, K, V, chunks = _layout(p.dtype, p.shape, p.stride(), None, None, None)
+        q_ptr, q_batch, q_row, given = 0, 0, 0, p
+    else:
+        B, K, V, chunks = _layout(p.dtype, p.shape, p.stride(), q.dtype, q.shape, q.stride())
+        q_ptr, (q_batch, q_row, _), given = q.data_ptr(), q.stride(), q
     _ints("verify_draft", "draft_tokens", draft_tokens, (B, K))
-    for name, t, shape in (("u", u, (B, K)), ("u_last", u_last, (B,))):
-        if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
-            raise ValueError(f"verify_draft: {name} must be contiguous f32 {list(shape)}")
+    if u.dtype is not torch.float32 or u.shape != (B, K) or not u.is_contiguous():
+        raise ValueError(f"verify_draft: u must be contiguous f32 [{B}, {K}]")
+    if u_last.dtype is not torch.float32 or u_last.shape != (B,) or not u_last.is_contiguous():
+        raise ValueError(f"verify_draft: u_last must be contiguous f32 [{B}]")
+    counted = u if counts is None else counts
     if counts is not None:
         _ints("verify_draft", "counts", counts, (B,))
-    dev, stream = _where("verify_draft", target_probs, draft_probs=draft_probs, draft_tokens=draft_tokens, u=u,
-                         u_last=u_last, counts=counts)
-    chunks = -(-V // lib.verify_chunk())
-    sums = torch.empty(B * chunks * 2, dtype=torch.float64, device=target_probs.device)
-    out = torch.empty(B * (K + 2), dtype=torch.int32, device=target_probs.device)
-    tokens, accepted = out[:B * (K + 1)].view(B, K + 1), out[B * (K + 1):]
-    q = draft_probs
-    lib.verify_draft(dev, stream, target_probs.data_ptr(), target_probs.stride(0), target_probs.stride(1),
-                     q.data_ptr() if q is not None and K else 0, q.stride(0) if q is not None else 0,
-                     q.stride(1) if q is not None else 0, draft_tokens.data_ptr(), u.data_ptr(), u_last.data_ptr(),
-                     counts.data_ptr() if counts is not None else 0, tokens.data_ptr(), accepted.data_ptr(),
-                     sums.data_ptr(), sums.numel() * 8, B, K, V, _ELEM[target_probs.dtype])
-    return tokens, accepted
+    dev, stream = _where("verify_draft", p, given, draft_tokens, u, u_last, counted)
+    # workspace and outputs in one allocation: f64 sums by chunk, tokens, accepted
+    sums = 2 * B * chunks
+    out = draft_tokens.new_empty((sums + B * (K + 2),))
+    _, tokens, accepted = out.split_with_sizes((sums, B * (K + 1), B))
+    p_batch, p_row, _ = p.stride()
+    lib.verify_draft(dev, stream, p.data_ptr(), p_batch, p_row, q_ptr, q_batch, q_row, draft_tokens.data_ptr(),
+                     u.data_ptr(), u_last.data_ptr(), 0 if counts is None else counts.data_ptr(), tokens.data_ptr(),
+                     accepted.data_ptr(), out.data_ptr(), B, K, V, _ELEM[p.dtype])
+    return tokens.view(B, K + 1), accepted
