@@ -166,12 +166,14 @@ __device__ __forceinline__ Request request_of(const PagedAttnArgs& a, uint32_t b
   return r;
 }
 
-// Keys of one split: whole blocks of 32, at least kMinSplit keys, so that short
+// Keys of one split: whole tiles of 64 (two blocks of the few-row body), so that no
+// tile reaches into the next split's keys; at least kMinSplit, so that short
 // requests use few of the launch's splits.
+constexpr int32_t kManyKeys = 64;   // keys of a K / V tile of the many-row body
 constexpr int32_t kMinSplit = 256;
 __device__ __forceinline__ int32_t split_keys(int32_t kv, uint32_t splits) {
   const int32_t per = (int32_t)(((uint32_t)kv + splits - 1) / splits);
-  return max((per + 31) & ~31, kMinSplit);
+  return max((per + kManyKeys - 1) & ~(kManyKeys - 1), kMinSplit);
 }
 __device__ __forceinline__ int32_t splits_used(int32_t kv, int32_t per) { return max((kv + per - 1) / per, 1); }
 
@@ -244,9 +246,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
       const int32_t t = c0 + ((n0 + (int32_t)(lane >> 1)) * kFewWaves + (int32_t)wave) * 32 + 16 * (int32_t)(lane & 1);
       ids = t < c1 ? table[t >> a.page_shift] : 0;
     };
-    // The block ahead of the one multiplied, in registers. (Two were tried for 4
-    // column blocks, where a SIMD holds one wave: 150 registers spill and 32 x 5
-    // rows take 84 us, not 44.)
+    // The block ahead of the one multiplied, in registers.
     u32x4 kr[2 * LD], vr[2 * LD];
     bool missing[2] = {};
     auto load = [&](int32_t n) {
@@ -458,7 +458,6 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
 
 // ---------------------------------------------------------------- many rows
 constexpr int kManyRows = 128;  // rows of a workgroup's tile: 4 waves of 32
-constexpr int kManyKeys = 64;   // keys of a K / V tile
 
 // Tile x of all tiles of the requests with more than few_rows rows, the last
 // request's last tile first (of a prompt's tiles the last sees the most keys).
@@ -496,6 +495,16 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, uint32_t x, ui
 // not follow: probabilities may reach 2^kLazy, and rescaling O becomes rare
 // after the first tiles. fp16: 2^(kLazy + shift) stays below 65504.
 constexpr float kLazy = 6.f;
+
+// A wave owns 32 rows, the workgroup walks tiles of 64 keys in two LDS buffers:
+// tile i + 1 flies into registers while tile i is multiplied, one barrier a tile
+// (a buffer is written two tiles after it was read). 4096 rows behind 4095 cached
+// keys of the 8B heads: 417 us, 990 TFLOP/s, where the library's 8192^3 product
+// of such values reaches 1140 - 1230 on this card. The wave alternates between
+// the matrix cores (1024 cycles a tile) and the vector ALU (1000, half of it
+// exponentials); two workgroups a CU overlap them in part. Tried and not kept:
+// 64 rows a wave (half the LDS reads, one wave per SIMD: 675 us); 32-key steps
+// with the next scores beside the exponentials (444).
 
 template <typename T, int HD>
 __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds, uint32_t x, uint32_t kvh, uint32_t split) {
@@ -557,25 +566,31 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
   const uint32_t vread = kV + (4 * half + ((lane & 15) >> 2)) * kVRow<HD> + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const uint32_t mine = (tid / (HD / 8)) % 16 * HD + tid % (HD / 8) * 8;  // in its group of 16 keys
 
-  int32_t ids = 0;  // page of the lane's group of 16 keys, for 16 tiles
+  // Where the lane's group of 16 keys (one page) begins, for 16 tiles. A group
+  // whose page is outside the pool reads page 0; the first such key makes the
+  // rows that see it NaN.
+  int32_t first_missing = rq.kv > rq.cap ? 0 : kNever;
+  uint32_t at_lo = 0, at_hi = 0;
+  auto find_groups = [&](int32_t i) {
+    const int32_t t = c0 + i * kManyKeys + 16 * (int32_t)lane;
+    int32_t page = t < c1 ? table[t >> a.page_shift] : 0;
+    const uint64_t outside = __ballot((uint32_t)page >= a.num_pages);
+    if (outside) first_missing = min(first_missing, c0 + i * kManyKeys + 16 * (int32_t)__builtin_ctzll(outside));
+    if ((uint32_t)page >= a.num_pages) page = 0;
+    const uint64_t at = (uint64_t)page * a.page_stride + (uint64_t)((uint32_t)t & ((1u << a.page_shift) - 1u)) * HD;
+    at_lo = (uint32_t)at;
+    at_hi = (uint32_t)(at >> 32);
+  };
   u32x4 kr[LJ], vr[LJ];
-  uint32_t next_miss = 0, miss = 0;  // groups of the tile whose page is outside the pool
   auto load = [&](int32_t i) {
-    if ((i & 15) == 0) {
-      const int32_t t = c0 + i * kManyKeys + 16 * (int32_t)lane;
-      ids = t < c1 ? table[t >> a.page_shift] : 0;
-    }
-    const uint64_t out = __ballot((uint32_t)ids >= a.num_pages);
-    next_miss = (uint32_t)(out >> (4 * (i & 15))) & 15u;
+    if ((i & 15) == 0) find_groups(i);
 #pragma unroll
     for (int j = 0; j < LJ; ++j) {
-      const uint32_t grp = (j * 256 + wave * 64) / (HD / 8) / 16;  // wave-uniform: 16 keys, one page
-      int32_t page = __builtin_amdgcn_readlane(ids, 4 * (i & 15) + grp);
-      if ((uint32_t)page >= a.num_pages) page = 0;
-      const uint32_t at = (uint32_t)(c0 + i * kManyKeys + 16 * (int32_t)grp) & ((1u << a.page_shift) - 1u);
-      const uint16_t* src = kbase + (uint64_t)page * a.page_stride + (uint64_t)at * HD;
-      kr[j] = *reinterpret_cast<const u32x4*>(src + mine);
-      vr[j] = *reinterpret_cast<const u32x4*>(src + a.kv_stride + mine);
+      const uint32_t grp = 4 * (i & 15) + (j * 256 + wave * 64) / (HD / 8) / 16;  // wave-uniform
+      const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_lo, grp) |
+                          (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_hi, grp) << 32;
+      kr[j] = *reinterpret_cast<const u32x4*>(kbase + at + mine);
+      vr[j] = *reinterpret_cast<const u32x4*>(kbase + a.kv_stride + at + mine);
     }
   };
   const int32_t tiles = (c1 - c0 + kManyKeys - 1) / kManyKeys;
@@ -607,12 +622,14 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
         take_special<T, HD>(reinterpret_cast<u32x4*>(buf + vw + j * (2048 / HD) * kVRow<HD>),
                             t0 + j * (2048 / HD) + (int32_t)(tid / (HD / 8)), tid % (HD / 8) * 8, first_key);
     }
-    miss = next_miss;
     if (i + 1 < tiles) load(i + 1);
     // the other buffer's readers passed the barrier of the tile before
     __syncthreads();
     if (t0 > wlast) continue;  // none of this wave's rows sees the tile
 
+    // Between the barrier and the last product a wave goes before those that load
+    // and store (430 -> 421 us for the 4096 rows, 52 -> 49 for 12 x 400 64-wide).
+    __builtin_amdgcn_s_setprio(1);
     f32x16_t s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -631,13 +648,6 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     // register e of s[t] is key 32 t + 8 (e / 4) + 4 half + e % 4
-    if (miss) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (miss >> (2 * t + e / 8) & 1) s[t][e] = __builtin_nanf("");
-    }
     if (t0 + kManyKeys - 1 > wfirst) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -702,9 +712,11 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
   }
   l += __shfl_xor(l, 32, 64);
   if (!in) return;
+  if (pos >= first_missing) l = __builtin_nanf("");
   if (tiles > 0 && special_s)  // set before the last tile's barrier
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -712,17 +724,15 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
       for (int e = 0; e < 16; ++e)
         o[d][e] = special<HD>(o[d][e], pos, 32 * d + 8 * (e / 4) + 4 * half + e % 4, first_key);
   if (used == 1) {
-    const float inv = 1.f / l;
+    // a row that sees nothing is 0; one that saw only -inf is NaN
+    const float inv = pos < 0 && !bad ? 0.f : l == 0.f ? __builtin_nanf("") : 1.f / l;
     uint16_t* dst = a.out + (uint64_t)(rq.row0 + tok) * a.out_stride + (uint64_t)(kvh * g + h) * HD + 4 * half;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[j] = bad || (l == 0.f && pos >= 0) ? __builtin_nanf("") : pos < 0 ? 0.f : o[d][e + j] * inv;
-        *reinterpret_cast<u32x2*>(dst + 32 * d + 2 * e) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+        *reinterpret_cast<u32x2*>(dst + 32 * d + 2 * e) = u32x2{pack2<T>(o[d][e] * inv, o[d][e + 1] * inv),
+                                                                pack2<T>(o[d][e + 2] * inv, o[d][e + 3] * inv)};
       }
   } else {
     const uint64_t at = a.plan.few_part + (((uint64_t)x * a.hkv + kvh) * a.plan.many_splits + split) * kManyRows + wave * 32 + col;
@@ -740,7 +750,7 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
 }
 
 template <typename T, int HD, int NB>
-__global__ void __launch_bounds__(64 * kFewWaves, NB == 4 ? 1 : 2) k_paged_few(PagedAttnArgs a) {
+__global__ void __launch_bounds__(64 * kFewWaves, 2) k_paged_few(PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[kFewWaves * 32 * kKVRow<HD>];
   few_body<T, HD, NB>(a, lds, blockIdx.z, blockIdx.x, blockIdx.y);
 }
@@ -748,7 +758,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, NB == 4 ? 1 : 2) k_paged_few(P
 // Both kinds of requests in one launch: the long tiles first, then the few-row
 // requests, which fill in beside them.
 template <typename T, int HD, int NB>
-__global__ void __launch_bounds__(256, NB == 4 ? 1 : 2) k_paged_mixed(PagedAttnArgs a) {
+__global__ void __launch_bounds__(256, 2) k_paged_mixed(PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kManyKeys * kKVRow<HD>];
   uint32_t i = blockIdx.x;
   const uint32_t kvh = i % a.hkv;  // a head's workgroups share their K and V, and with 8 heads an XCD's L2
@@ -762,88 +772,90 @@ __global__ void __launch_bounds__(256, NB == 4 ? 1 : 2) k_paged_mixed(PagedAttnA
   }
 }
 
-// Joins the splits of a row: one wave per row, HD / 64 dims a lane. The first
-// many_tiles blocks of rows are those of the tiles, then each request's few rows.
+// Joins the splits: a thread adds four dims of kJoin rows over the splits, with a
+// running maximum, four splits' loads in flight. A workgroup takes a part of one
+// unit - a tile of many rows, or the rows of a request of few - and the units'
+// first blocks are those of the tiles.
+constexpr uint32_t kJoin = 4;
+template <int HD>
+constexpr uint32_t join_parts(uint32_t rows) { return (rows * (HD / 4) + 256 * kJoin - 1) / (256 * kJoin); }
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) k_paged_combine(PagedAttnArgs a) {
-  constexpr int E = HD / 64;
-  const uint32_t lane = threadIdx.x & 63, kvh = blockIdx.y;
+  const uint32_t kvh = blockIdx.y;
   const uint32_t g = a.hq / a.hkv;
-  const uint32_t many_groups = a.plan.many_splits > 1 ? a.plan.many_tiles * (kManyRows / 4) : 0;
-  uint32_t b, splits, R;
-  int32_t r, keys;  // row of the request, keys that were split
+  const uint32_t many_blocks = a.plan.many_splits > 1 ? a.plan.many_tiles * join_parts<HD>(kManyRows) : 0;
+  uint32_t b, splits, R, part;
+  int32_t r0, keys;  // first row of the unit in its request, keys that were split
   uint64_t at;
   Request rq;
-  if (blockIdx.x < many_groups) {
-    const uint32_t x = blockIdx.x / (kManyRows / 4), rr = (blockIdx.x % (kManyRows / 4)) * 4 + wave_id();
+  if (blockIdx.x < many_blocks) {
+    const uint32_t x = blockIdx.x / join_parts<HD>(kManyRows);
+    part = blockIdx.x % join_parts<HD>(kManyRows);
     int32_t ti;
     if (!find_tile(a, x, &b, &ti)) return;
     rq = request_of(a, b);
-    const int32_t rows = rq.n * (int32_t)g, r0 = ti * kManyRows;
-    r = r0 + (int32_t)rr;
-    if (r >= rows) return;
-    keys = max(rq.kv - rq.n + (min(r0 + kManyRows, rows) - 1) / (int32_t)g + 1, 0);
+    r0 = ti * kManyRows;
+    keys = max(rq.kv - rq.n + (min(r0 + kManyRows, rq.n * (int32_t)g) - 1) / (int32_t)g + 1, 0);
     splits = a.plan.many_splits;
     R = kManyRows;
-    at = a.plan.few_part + ((uint64_t)x * a.hkv + kvh) * splits * R + rr;
+    at = a.plan.few_part + ((uint64_t)x * a.hkv + kvh) * splits * R;
   } else {
-    const uint32_t i = blockIdx.x - many_groups;
+    const uint32_t i = blockIdx.x - many_blocks;
     R = 16 * a.plan.few_blocks;
-    b = i / (R / 4);
-    const uint32_t rr = (i % (R / 4)) * 4 + wave_id();
+    b = i / join_parts<HD>(R);
+    part = i % join_parts<HD>(R);
     rq = request_of(a, b);
-    const int32_t rows = rq.n * (int32_t)g;
-    r = (int32_t)rr;
-    if (r >= rows || rows > (int32_t)R) return;
+    if (rq.n * (int32_t)g > (int32_t)R) return;
+    r0 = 0;
     keys = rq.kv;
     splits = a.plan.few_splits;
-    at = ((uint64_t)b * a.hkv + kvh) * splits * R + rr;
+    at = ((uint64_t)b * a.hkv + kvh) * splits * R;
   }
   if (rq.kv > rq.cap) return;
   const int32_t used = splits_used(keys, split_keys(keys, splits));
   if (used == 1) return;
-  // lane: split s0 + lane. Its weight is broadcast while the wave adds the splits'
-  // rows, eight loads in flight.
-  float big = -__builtin_inff(), sum = 0.f, o[E] = {};
-  for (int32_t s0 = 0; s0 < used; s0 += 64) {
-    const int32_t left = min(used - s0, 64);
-    const bool on = (int32_t)lane < left;
-    const uint64_t i = at + (uint64_t)(s0 + (on ? (int32_t)lane : 0)) * R;
-    const float m = on ? a.part_ml[2 * i] : -__builtin_inff(), l = on ? a.part_ml[2 * i + 1] : 0.f;
-    float mx = m;
+  const int32_t rows = rq.n * (int32_t)g;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-    mx = fmaxf(mx, big);
-    const float old = big == mx ? 1.f : big == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(big - mx);
-    const float f = m == mx ? 1.f : m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-    float ls = on ? f * l : 0.f;
+  for (uint32_t u = 0; u < kJoin; ++u) {
+    const uint32_t item = (part * kJoin + u) * 256 + threadIdx.x, rr = item / (HD / 4), d = item % (HD / 4) * 4;
+    const int32_t r = r0 + (int32_t)rr;
+    if (rr >= R || r >= rows) continue;
+    float big = -__builtin_inff(), sum = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int32_t s = 0; s < used; s += 4) {
+      float m[4], l[4];
+      f32x4_t x[4];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) ls += __shfl_xor(ls, d, 64);
-    sum = sum * old + ls;
-    big = mx;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= old;
-    const float* po = a.part_o + (at + (uint64_t)s0 * R) * HD + lane * E;
-    for (int32_t s = 0; s < left; s += 8) {
-      float x[8][E];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[u][e] = po[(uint64_t)min(s + u, left - 1) * R * HD + e];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s + u, left - 1)));
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (s + u < left) o[e] += w * x[u][e];
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t i = at + rr + (uint64_t)min(s + e, used - 1) * R;
+        m[e] = a.part_ml[2 * i];
+        l[e] = a.part_ml[2 * i + 1];
+        x[e] = *reinterpret_cast<const f32x4_t*>(a.part_o + i * HD + d);
       }
-    }
-  }
-  const uint32_t tok = (uint32_t)r / g, h = (uint32_t)r - tok * g;
-  const bool none = rq.kv - rq.n + (int32_t)tok < 0;
-  T* out = reinterpret_cast<T*>(a.out) + (uint64_t)(rq.row0 + tok) * a.out_stride + (uint64_t)(kvh * g + h) * HD;
+      float mx = big;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[lane * E + e] = from_f32<T>(none ? 0.f : o[e] / sum);
+      for (int e = 0; e < 4; ++e) mx = max2(mx, m[e]);
+      const float old = big == mx ? 1.f : big == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(big - mx);
+      sum *= old;
+      o *= old;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float f = s + e >= used ? 0.f : m[e] == mx ? 1.f : m[e] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[e] - mx);
+        if (s + e < used) {
+          sum += f * l[e];
+          o += f * x[e];
+        }
+      }
+      big = mx;
+    }
+    const uint32_t tok = (uint32_t)r / g, h = (uint32_t)r - tok * g;
+    const float inv = rq.kv - rq.n + (int32_t)tok < 0 ? 0.f : 1.f / sum;
+    uint16_t* out = a.out + (uint64_t)(rq.row0 + tok) * a.out_stride + (uint64_t)(kvh * g + h) * HD + d;
+    // sum 0: the row saw only scores of -inf, 0 / 0
+    if (sum == 0.f && inv != 0.f) o = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+    *reinterpret_cast<u32x2*>(out) = u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+  }
 }
 
 template <typename T, int HD, int NB>
@@ -856,8 +868,8 @@ hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t s) {
   } else {
     hipLaunchKernelGGL((k_paged_few<T, HD, NB>), dim3(a.hkv, p.few_splits, a.B), dim3(64 * kFewWaves), 0, s, a);
   }
-  const uint64_t groups = (p.many_splits > 1 ? (uint64_t)p.many_tiles * (kManyRows / 4) : 0) +
-                          (p.few_splits > 1 ? (uint64_t)a.B * 4 * NB : 0);
+  const uint64_t groups = (p.many_splits > 1 ? (uint64_t)p.many_tiles * join_parts<HD>(kManyRows) : 0) +
+                          (p.few_splits > 1 ? (uint64_t)a.B * join_parts<HD>(16 * NB) : 0);
   if (groups > INT32_MAX) return hipErrorInvalidValue;
   if (groups) hipLaunchKernelGGL((k_paged_combine<T, HD>), dim3((uint32_t)groups, a.hkv), dim3(256), 0, s, a);
   return hipGetLastError();
@@ -865,12 +877,8 @@ hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t s) {
 
 template <typename T>
 hipError_t launch_attn_of(const PagedAttnArgs& a, hipStream_t s) {
-#define OGKM_ATTN_NB(HD)                                              \
-  (a.plan.few_blocks == 1   ? launch_attn<T, HD, 1>(a, s)             \
-   : a.plan.few_blocks == 2 ? launch_attn<T, HD, 2>(a, s)             \
-                            : launch_attn<T, HD, 4>(a, s))
-  return a.hd == 128 ? OGKM_ATTN_NB(128) : OGKM_ATTN_NB(64);
-#undef OGKM_ATTN_NB
+  if (a.hd == 128) return a.plan.few_blocks == 1 ? launch_attn<T, 128, 1>(a, s) : launch_attn<T, 128, 2>(a, s);
+  return a.plan.few_blocks == 1 ? launch_attn<T, 64, 1>(a, s) : launch_attn<T, 64, 2>(a, s);
 }
 
 }  // namespace
@@ -880,26 +888,30 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
   PagedAttnPlan p{};
   const uint64_t g = hq / hkv, most = std::min(max_q, n) * g;  // rows of a request, at most
   const uint64_t heads = hkv, key_splits = std::max<uint64_t>((max_kv + kMinSplit - 1) / kMinSplit, 1);
-  const uint64_t few = most <= 64 ? most : g;  // rows that the few-row body is laid out for
-  p.few_blocks = few <= 16 ? 1 : few <= 32 ? 2 : 4;
+  // Up to 32 rows: the few-row body. (With 4 column blocks, up to 64, it needs all
+  // 512 registers: 32 x 5 drafted rows of 8 heads at up to 8191 keys took 48 us,
+  // the other body's half-empty tiles take 38.)
+  const bool only_few = most <= 32;
+  const uint64_t few = only_few ? most : g;  // rows that the few-row body is laid out for
+  p.few_blocks = few <= 16 ? 1 : 2;
   p.many_splits = 1;
-  if (most <= 64) {
+  if (only_few) {
     p.few_rows = INT32_MAX;  // a request beyond the host's bound is taken tile by tile
   } else {
-    // 0 rows where one token already fills the tiles
-    p.few_rows = g <= 64 ? 16 * p.few_blocks : 0;
+    // 0 rows where one token already takes more
+    p.few_rows = g <= 32 ? 16 * p.few_blocks : 0;
     p.many_tiles = (uint32_t)(n * g / kManyRows + std::min<uint64_t>(B, n * g / (p.few_rows + 1)));
+    // Two workgroups a CU. us at 256 / 512 / 1024 workgroups: 512 rows behind 4096
+    // keys (8B heads) 67 / 58 / 70, 48 mixed requests of 64-wide heads 51 / 51 / 61.
     const uint64_t wgs = std::max<uint64_t>(p.many_tiles * heads, 1);
-    // two workgroups a CU; more splits only add partial results (48 mixed
-    // requests of 64-wide heads: 55 us at 512, 91 at 1024)
     p.many_splits = (uint32_t)std::min<uint64_t>((512 + wgs - 1) / wgs, key_splits);
   }
-  const uint64_t wgs = std::max<uint64_t>(B * heads, 1);
   // A workgroup a CU: four waves with a block each in flight draw what HBM gives.
   // us at 128 / 256 / 512 / 1024 workgroups: 4 requests of up to 131071 keys 343 /
   // 257 / 257 / 257, 16 of 4096 49 / 42 / 44 / 44, 64 of 2048 (70B heads) 70 / 70 /
-  // 70 / 78, 32 x 5 rows of 8191 (one kv head) 126 / 44 / 58 / 82. At least kMinSplit keys
-  // each: 128, 256 and 512 are within 2 us, 1024 loses 3 on 4 requests of 8192.
+  // 70 / 78. At least kMinSplit keys each: 128, 256 and 512 are within 2 us, 1024
+  // loses 3 on 4 requests of 8192.
+  const uint64_t wgs = std::max<uint64_t>(B * heads, 1);
   p.few_splits = (uint32_t)std::min<uint64_t>((256 + wgs - 1) / wgs, key_splits);
   p.few_part = p.few_splits > 1 ? wgs * p.few_splits * 16 * p.few_blocks : 0;
   p.part_rows = p.few_part + (p.many_splits > 1 ? p.many_tiles * heads * p.many_splits * kManyRows : 0);

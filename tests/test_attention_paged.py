@@ -374,6 +374,16 @@ def test_attention_long_gpu(gpu_rt, dt, ql, kl):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 1, 128), (16, 2, 64)])
+@pytest.mark.parametrize("ql,kl", [([5, 5, 5], [8191, 3003, 777]), ([5, 1, 7], [4200, 4300, 1111]), ([70], [5000])])
+def test_attention_split_tiles_gpu(gpu_rt, dt, hq, hkv, hd, ql, kl):
+    """More rows than the few-row body takes, over keys that are split: the splits'
+    shares of such lengths are not whole 64-key tiles by themselves."""
+    _check_attn(True, dt, ql, kl, hq, hkv, hd, 32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("sharp", [0.0, 30.0])
 def test_attention_flat_and_peaked_gpu(gpu_rt, sharp):
     """All scores equal; scores whose maximum moves far from tile to tile."""
