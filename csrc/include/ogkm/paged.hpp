@@ -55,6 +55,7 @@ struct PagedRopeArgs {
 struct PagedAttnPlan {
   uint32_t few_rows;    // requests of up to so many rows per kv head take the `few` body
   uint32_t few_blocks;  // its column blocks of 16 rows: 1 or 2
+  uint32_t few_waves;   // waves of a workgroup: 4 or 8
   uint32_t few_splits;  // its splits of the key axis, at most
   uint32_t many_tiles;  // 128-row tiles of the other requests, at most (0: none expected)
   uint32_t many_splits;

@@ -178,9 +178,8 @@ __device__ __forceinline__ int32_t split_keys(int32_t kv, uint32_t splits) {
 __device__ __forceinline__ int32_t splits_used(int32_t kv, int32_t per) { return max((kv + per - 1) / per, 1); }
 
 // ---------------------------------------------------------------- few rows
-constexpr int kFewWaves = 4;
 
-template <typename T, int HD, int NB>
+template <typename T, int HD, int NB, int NW>
 __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, uint32_t b, uint32_t kvh, uint32_t split) {
   constexpr int KS = HD / 32, DT = HD / 16, LD = HD / 32;  // k steps, dim tiles, loads per 16 rows
   constexpr int R = 16 * NB;
@@ -201,9 +200,9 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
   uint16_t* vw = lds + wave * (32 * kKVRow<HD>) + 32 * kKRow<HD> + (lane / (HD / 8)) * kVRow<HD> + (lane % (HD / 8)) * 8;
   const uint16_t* kread = lds + wave * (32 * kKVRow<HD>) + col * kKRow<HD> + 8 * quad;
   const uint16_t* vread = lds + wave * (32 * kKVRow<HD>) + 32 * kKRow<HD> + (4 * quad + (col >> 2)) * kVRow<HD> + 4 * (col & 3);
-  __shared__ float wm[kFewWaves][R], wl[kFewWaves][R];
-  __shared__ int32_t first_key[kFewWaves][3 * HD];  // take_special; set only by a wave that met one
-  __shared__ uint32_t special_s[kFewWaves];
+  __shared__ float wm[NW][R], wl[NW][R];
+  __shared__ int32_t first_key[NW][3 * HD];  // take_special; set only by a wave that met one
+  __shared__ uint32_t special_s[NW];
   const uint16_t* kbase = a.pages + kvh * a.head_stride;
   const int32_t* table = a.table + b * a.table_ld;
   const float c = a.scale * 1.44269504088896340736f;  // scores in powers of two
@@ -240,10 +239,10 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
     bool wave_special = false;
     // Page ids of this wave's next 32 blocks, one half block per lane (a page
     // holds at least 16 tokens), so that a block's addresses are wave-uniform.
-    const int32_t mine = (blocks - (int32_t)wave + kFewWaves - 1) / kFewWaves;
+    const int32_t mine = (blocks - (int32_t)wave + NW - 1) / NW;
     int32_t ids = 0;
     auto fetch_ids = [&](int32_t n0) {
-      const int32_t t = c0 + ((n0 + (int32_t)(lane >> 1)) * kFewWaves + (int32_t)wave) * 32 + 16 * (int32_t)(lane & 1);
+      const int32_t t = c0 + ((n0 + (int32_t)(lane >> 1)) * NW + (int32_t)wave) * 32 + 16 * (int32_t)(lane & 1);
       ids = t < c1 ? table[t >> a.page_shift] : 0;
     };
     // The block ahead of the one multiplied, in registers.
@@ -252,7 +251,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
     auto load = [&](int32_t n) {
       if (n >= mine) return;
       if ((n & 31) == 0) fetch_ids(n);
-      const int32_t t0 = c0 + (n * kFewWaves + (int32_t)wave) * 32;
+      const int32_t t0 = c0 + (n * NW + (int32_t)wave) * 32;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         int32_t page = __builtin_amdgcn_readlane(ids, 2 * (n & 31) + h);
@@ -271,7 +270,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
     load(0);
     for (int32_t n = 0; n < mine; ++n) {
       const bool miss0 = missing[0], miss1 = missing[1];
-      const int32_t t0 = c0 + (n * kFewWaves + (int32_t)wave) * 32;
+      const int32_t t0 = c0 + (n * NW + (int32_t)wave) * 32;
       const bool masked = t0 + 31 > first;
       bool odd = false;
       if (masked) {
@@ -365,8 +364,8 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
-    // Join the waves: maxima through LDS, then two rounds of adding halves
-    // (waves 2, 3 -> 0, 1; wave 1 -> 0), f32 in the K / V space.
+    // Join the waves: maxima through LDS, then rounds in which the upper half of
+    // the waves left is added to the lower, f32 in the K / V space.
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       l[nb] += __shfl_xor(l[nb], 16, 64);
@@ -382,10 +381,12 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const uint32_t r = nb * 16 + col;
-      big[nb] = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+      big[nb] = -__builtin_inff();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) big[nb] = fmaxf(big[nb], wm[w][r]);
       sum[nb] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float f = wm[w][r] == -__builtin_inff() ? (big[nb] == wm[w][r] ? 1.f : 0.f)
                                                       : __builtin_amdgcn_exp2f(wm[w][r] - big[nb]);
         sum[nb] += f * wl[w][r];
@@ -394,7 +395,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
           for (int d = 0; d < DT; ++d) o[nb][d] *= f;
       }
     }
-    float* ox = reinterpret_cast<float*>(lds);  // [2][R][HD]; the lanes' own order, 16 bytes each
+    float* ox = reinterpret_cast<float*>(lds);  // [NW / 2][R][HD]; the lanes' own order, 16 bytes each
     auto put = [&](float* at) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
@@ -407,15 +408,15 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[nb][d] += *reinterpret_cast<const f32x4_t*>(at + ((nb * DT + d) * 64 + lane) * 4);
     };
-    if (wave >= 2) put(ox + (wave - 2) * R * HD);
-    __syncthreads();
-    if (wave < 2) add(ox + wave * R * HD);
-    __syncthreads();
-    if (wave == 1) put(ox);
-    __syncthreads();
+#pragma unroll 1
+    for (uint32_t left = NW / 2; left; left /= 2) {
+      if (wave >= left && wave < 2 * left) put(ox + (wave - left) * R * HD);
+      __syncthreads();
+      if (wave < left) add(ox + wave * R * HD);
+      __syncthreads();
+    }
     if (wave == 0) {
-      add(ox);
-      for (int w = 0; w < kFewWaves; ++w)
+      for (int w = 0; w < NW; ++w)
         if (special_s[w])
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
@@ -452,7 +453,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
         }
       }
     }
-    if (looped) __syncthreads();  // the next tile writes the LDS again
+    if (looped) __syncthreads();  // wave 0 still reads what the next tile writes
   }
 }
 
@@ -749,10 +750,10 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
   }
 }
 
-template <typename T, int HD, int NB>
-__global__ void __launch_bounds__(64 * kFewWaves, 2) k_paged_few(PagedAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[kFewWaves * 32 * kKVRow<HD>];
-  few_body<T, HD, NB>(a, lds, blockIdx.z, blockIdx.x, blockIdx.y);
+template <typename T, int HD, int NB, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) k_paged_few(PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[NW * 32 * kKVRow<HD>];
+  few_body<T, HD, NB, NW>(a, lds, blockIdx.z, blockIdx.x, blockIdx.y);
 }
 
 // Both kinds of requests in one launch: the long tiles first, then the few-row
@@ -768,7 +769,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_mixed(PagedAttnArgs a) {
     many_body<T, HD>(a, lds, i / a.plan.many_splits, kvh, i % a.plan.many_splits);
   } else {
     i -= many;
-    few_body<T, HD, NB>(a, lds, i / a.plan.few_splits, kvh, i % a.plan.few_splits);
+    few_body<T, HD, NB, 4>(a, lds, i / a.plan.few_splits, kvh, i % a.plan.few_splits);
   }
 }
 
@@ -866,7 +867,11 @@ hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t s) {
     if (wgs > INT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_paged_mixed<T, HD, NB>), dim3((uint32_t)wgs), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((k_paged_few<T, HD, NB>), dim3(a.hkv, p.few_splits, a.B), dim3(64 * kFewWaves), 0, s, a);
+    const dim3 grid(a.hkv, p.few_splits, a.B);
+    if (p.few_waves == 8)
+      hipLaunchKernelGGL((k_paged_few<T, HD, NB, 8>), grid, dim3(512), 0, s, a);
+    else
+      hipLaunchKernelGGL((k_paged_few<T, HD, NB, 4>), grid, dim3(256), 0, s, a);
   }
   const uint64_t groups = (p.many_splits > 1 ? (uint64_t)p.many_tiles * join_parts<HD>(kManyRows) : 0) +
                           (p.few_splits > 1 ? (uint64_t)a.B * join_parts<HD>(16 * NB) : 0);
@@ -901,10 +906,12 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
     // 0 rows where one token already takes more
     p.few_rows = g <= 32 ? 16 * p.few_blocks : 0;
     p.many_tiles = (uint32_t)(n * g / kManyRows + std::min<uint64_t>(B, n * g / (p.few_rows + 1)));
-    // Two workgroups a CU. us at 256 / 512 / 1024 workgroups: 512 rows behind 4096
-    // keys (8B heads) 67 / 58 / 70, 48 mixed requests of 64-wide heads 51 / 51 / 61.
+    // A workgroup a CU; the joining of more splits costs more than they save. us at
+    // 128 / 256 / 512 / 1024 workgroups: 512 rows behind 3584 keys (8B heads) 93 /
+    // 64 / 58 / 72, 1040 behind 1407 (8 heads, one kv head) 41 / 31 / 40 / 41, 15
+    // requests of 419 rows 55 / 53 / 74 / 78, 16 behind 32752 56 / 49 / 69 / 115.
     const uint64_t wgs = std::max<uint64_t>(p.many_tiles * heads, 1);
-    p.many_splits = (uint32_t)std::min<uint64_t>((512 + wgs - 1) / wgs, key_splits);
+    p.many_splits = (uint32_t)std::min<uint64_t>((256 + wgs - 1) / wgs, key_splits);
   }
   // A workgroup a CU: four waves with a block each in flight draw what HBM gives.
   // us at 128 / 256 / 512 / 1024 workgroups: 4 requests of up to 131071 keys 343 /
@@ -913,6 +920,14 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
   // loses 3 on 4 requests of 8192.
   const uint64_t wgs = std::max<uint64_t>(B * heads, 1);
   p.few_splits = (uint32_t)std::min<uint64_t>((256 + wgs - 1) / wgs, key_splits);
+  // Short contexts of few requests: eight waves and no second launch. us with it /
+  // with splits: one request of the 8B heads at 512 keys 9.4 / 11.8, at 1025 12.4 /
+  // 11.8, at 1536 15.1 / 11.6; 4 requests of 64-wide heads at 1025 8.9 / 11.6.
+  p.few_waves = 4;
+  if (only_few && p.few_splits > 1 && (uint64_t)max_kv * hd <= 96 * 1024) {
+    p.few_waves = 8;
+    p.few_splits = 1;
+  }
   p.few_part = p.few_splits > 1 ? wgs * p.few_splits * 16 * p.few_blocks : 0;
   p.part_rows = p.few_part + (p.many_splits > 1 ? p.many_tiles * heads * p.many_splits * kManyRows : 0);
   return p;
