@@ -462,32 +462,46 @@ constexpr int kManyRows = 128;  // rows of a workgroup's tile: 4 waves of 32
 
 // Tile x of all tiles of the requests with more than few_rows rows, the last
 // request's last tile first (of a prompt's tiles the last sees the most keys).
-// Every wave scans the request lengths by itself. Returns false past the end.
+// Every wave scans the request lengths by itself, 256 a round. Returns false past
+// the end.
 __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, uint32_t x, uint32_t* b, int32_t* tile) {
+  constexpr int E = 4;  // requests of a lane: top - 1 - E lane - e
   const uint32_t lane = threadIdx.x & 63;
-  const int32_t g = (int32_t)(a.hq / a.hkv);
-  for (int32_t top = (int32_t)a.B; top > 0; top -= 64) {  // lane: request top - 1 - lane
-    const int32_t r = top - 1 - (int32_t)lane;
-    uint32_t tiles = 0;
-    if (r >= 0) {
-      const int32_t lo = min(max(a.cu_q[r], 0), (int32_t)a.n), hi = min(max(a.cu_q[r + 1], lo), (int32_t)a.n);
-      const uint32_t rows = (uint32_t)(hi - lo) * (uint32_t)g;
-      tiles = rows > a.plan.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
+  const uint32_t g = a.hq / a.hkv;
+  for (int32_t top = (int32_t)a.B; top > 0; top -= 64 * E) {
+    const int32_t r0 = top - 1 - E * (int32_t)lane;
+    int32_t cu[E + 1];  // of requests r0 + 1 - e; every index that exists is in bounds
+#pragma unroll
+    for (int e = 0; e <= E; ++e) cu[e] = a.cu_q[max(r0 + 1 - e, 0)];
+    uint32_t upto[E], sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int32_t lo = min(max(cu[e + 1], 0), (int32_t)a.n), hi = min(max(cu[e], lo), (int32_t)a.n);
+      const uint32_t rows = r0 - e >= 0 ? (uint32_t)(hi - lo) * g : 0;
+      sum += rows > a.plan.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
+      upto[e] = sum;
     }
-    uint32_t upto = tiles;
+    uint32_t before = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t y = __shfl_up(upto, o, 64);
-      if ((int)lane >= o) upto += y;
+      const uint32_t y = __shfl_up(before, o, 64);
+      if ((int)lane >= o) before += y;
     }
-    const uint64_t past = __ballot(upto > x);
+    const uint64_t past = __ballot(before > x);
     if (past) {
       const int l = __builtin_ctzll(past);
-      *b = (uint32_t)(top - 1 - l);
-      *tile = (int32_t)((uint32_t)__builtin_amdgcn_readlane((int)upto, l) - 1 - x);
-      return true;
+      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane((int)(before - sum), l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t end = from + (uint32_t)__builtin_amdgcn_readlane((int)upto[e], l);
+        if (end > x) {
+          *b = (uint32_t)(top - 1 - E * l - e);
+          *tile = (int32_t)(end - 1 - x);
+          return true;
+        }
+      }
     }
-    x -= (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    x -= (uint32_t)__builtin_amdgcn_readlane((int)before, 63);
   }
   return false;
 }
@@ -864,7 +878,7 @@ hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t s) {
   const PagedAttnPlan& p = a.plan;
   if (p.many_tiles) {
     const uint64_t wgs = ((uint64_t)p.many_tiles * p.many_splits + (uint64_t)a.B * p.few_splits) * a.hkv;
-    if (wgs > INT32_MAX) return hipErrorInvalidValue;
+    if (wgs >= (1u << 24)) return hipErrorInvalidValue;  // threads of a grid stay below 2^32
     hipLaunchKernelGGL((k_paged_mixed<T, HD, NB>), dim3((uint32_t)wgs), dim3(256), 0, s, a);
   } else {
     const dim3 grid(a.hkv, p.few_splits, a.B);
@@ -875,7 +889,7 @@ hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t s) {
   }
   const uint64_t groups = (p.many_splits > 1 ? (uint64_t)p.many_tiles * join_parts<HD>(kManyRows) : 0) +
                           (p.few_splits > 1 ? (uint64_t)a.B * join_parts<HD>(16 * NB) : 0);
-  if (groups > INT32_MAX) return hipErrorInvalidValue;
+  if (groups >= (1u << 24)) return hipErrorInvalidValue;
   if (groups) hipLaunchKernelGGL((k_paged_combine<T, HD>), dim3((uint32_t)groups, a.hkv), dim3(256), 0, s, a);
   return hipGetLastError();
 }

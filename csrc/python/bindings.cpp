@@ -1180,8 +1180,8 @@ PYBIND11_MODULE(_ogkm, m) {
                          uint32_t page_size, uint32_t width, float scale, uint32_t elem, uint32_t max_q,
                          uint32_t max_kv, uint64_t part, uint64_t part_bytes) {
     const uint32_t shift = page_shift_of(page_size, "paged_attn");
-    if (B > 65535 || hkv > 65535 || (uint64_t)width * page_size > (1u << 30))
-      throw StatusError("paged_attn: at most 65535 requests and kv heads, 2^30 tokens per request");
+    if (B > 65535 || hkv > 65535 || (uint64_t)width * page_size > (1u << 30) || (uint64_t)n * hq > INT32_MAX)
+      throw StatusError("paged_attn: at most 65535 requests and kv heads, 2^30 tokens per request, 2^31 - 1 rows x heads");
     if (!hkv || hq % hkv || (hd != 64 && hd != 128) || elem > ELEM_F16 || n > INT32_MAX)
       throw StatusError("paged_attn: hq % hkv, hd 64 or 128, bf16 or fp16");
     PagedAttnArgs a{(const uint16_t*)q, q_stride, q_head_stride, (const uint16_t*)pages, kv_stride, page_stride,

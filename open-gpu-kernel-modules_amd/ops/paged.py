@@ -235,8 +235,10 @@ def _attention_layout(dtype, q, q_stride, pool_dtype, pool, pool_stride, lens, t
         raise ValueError(f"attention: head dim 64 or 128, got {hd}")
     if len(q) != 3 or q[2] != hd or q[1] < 1 or q[1] % hkv:
         raise ValueError(f"attention: q must be [n, hq, {hd}] with hq a multiple of {hkv}")
-    if q_stride[2] != 1 or any(c > 1 and s % 8 for c, s in zip(q[:2], q_stride[:2])) or q[0] >= 2**31:
+    if q_stride[2] != 1 or any(c > 1 and s % 8 for c, s in zip(q[:2], q_stride[:2])):
         raise ValueError("attention: q's heads must be contiguous and 16-byte aligned")
+    if q[0] * q[1] >= 2**31:
+        raise ValueError("attention: fewer than 2^31 rows x heads")
     if len(lens) != 1 or lens[0] > 65535:
         raise ValueError("attention: kv_lens must list at most 65535 requests")
     _check_table("attention", table_dtype, table, table_stride, lens[0])

@@ -287,7 +287,7 @@ def _attn_oracle(q, pool, cu, kl, table, scale):
                 s = qq @ kk.T * scale
                 p = torch.softmax(s, -1)
                 r = p @ vv
-                ds = (hd + 4) * 2.0 ** -24 * (qq.abs() @ kk.abs().T * scale).amax(-1, keepdim=True)
+                ds = (hd + 4) * 2.0 ** -24 * (qq.abs() @ kk.abs().T * abs(scale)).amax(-1, keepdim=True)
                 o[t, h * g:(h + 1) * g] = r
                 tol[t, h * g:(h + 1) * g] = 1.05 * (e * r.abs() + (e + 2 * ds + 2.0 ** -20) * (p @ vv.abs())) + \
                     torch.finfo(q.dtype).tiny * e * 2
@@ -388,6 +388,80 @@ def test_attention_split_tiles_gpu(gpu_rt, dt, hq, hkv, hd, ql, kl):
 def test_attention_flat_and_peaked_gpu(gpu_rt, sharp):
     """All scores equal; scores whose maximum moves far from tile to tile."""
     _check_attn(True, torch.float16, [1, 40], [900, 700], 8, 2, 64, 32, sharp=sharp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(8, 1), (40, 1), (80, 2)])
+@pytest.mark.parametrize("B", [70, 300])
+def test_attention_many_requests_gpu(gpu_rt, B, hq, hkv):
+    """More requests than a wave finds in one round, some without rows; groups of more
+    heads than the few-row body takes."""
+    g = torch.Generator().manual_seed(B)
+    ql = [int(x) if x < 9 else 0 for x in torch.randint(0, 11, (B,), generator=g)]
+    ql[B // 3], ql[-1] = 40, 33
+    kl = [q + int(x) for q, x in zip(ql, torch.randint(0, 60, (B,), generator=g))]
+    _check_attn(True, torch.bfloat16, ql, kl, hq, hkv, 64, 16, extra_rows=1)
+
+
+def _check_scale(gpu, scale):
+    dev = _dev(gpu)
+    g = torch.Generator().manual_seed(6)
+    for ql, kl in (([1, 3], [70, 9]), ([50], [90])):
+        table, cu, num = _requests(ql, kl, 16)
+        q = torch.randn(cu[-1], 4, 64, generator=g).half()
+        pool = torch.randn(2, num, 2, 16, 64, generator=g).half()
+        want, tol = _attn_oracle(q, pool, cu, kl, table, scale)
+        # the bound's score term takes the scale's size
+        got = paged.attention(q.to(dev), pool.to(dev), _i32(cu, dev), _i32(kl, dev), table.to(dev), scale=scale)
+        assert ((got.cpu().double() - want).abs() <= tol.abs()).all()
+
+
+@pytest.mark.parametrize("scale", [0.3, -0.125, 1e-6])
+def test_attention_scale_cpu(fake_rt, scale):
+    _check_scale(False, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.3, -0.125, 1e-6])
+def test_attention_scale_gpu(gpu_rt, scale):
+    _check_scale(True, scale)
+
+
+def _check_infinite_scores(gpu, m, kv):
+    """An infinite k makes a score of plus or minus infinity by the sign of q there:
+    NaN, as inf - inf in the softmax, or a key that counts nothing; rows that see
+    only the latter are NaN (0 / 0)."""
+    dev = _dev(gpu)
+    g = torch.Generator().manual_seed(m)
+    hq, hd = 2, 64
+    table, cu, num = _requests([m], [kv], 16)
+    q = torch.randn(m, hq, hd, generator=g).bfloat16()
+    q[:, 0, 7] = -1.0
+    q[:, 1, 7] = 1.0
+    pool = torch.randn(2, num, 1, 16, hd, generator=g).bfloat16()
+    at = lambda t: (0, table[0, t // 16], 0, t % 16, 7)  # noqa: E731
+    pool[at(kv - m + 1)] = math.inf
+    pool[at(kv - 1)] = math.inf
+    if kv == m:  # the first row sees one key
+        pool[at(0)] = math.inf
+    want, tol = _attn_oracle(q, pool, cu, [kv], table, 0.125)
+    got = paged.attention(q.to(dev), pool.to(dev), _i32(cu, dev), _i32([kv], dev), table.to(dev)).cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    fine = ~want.isnan()
+    # ds of such rows is infinite: the score errors of the finite keys, |q| |k| sums of 64 terms, are below 1e-4
+    bound = tol.where(torch.isfinite(tol), 2.0 ** -8 * want.abs() + (2.0 ** -8 + 1e-3) * 5)
+    assert ((got - want).abs()[fine] <= bound[fine]).all()
+
+
+@pytest.mark.parametrize("m,kv", [(3, 3), (4, 40), (40, 70)])
+def test_attention_infinite_scores_cpu(fake_rt, m, kv):
+    _check_infinite_scores(False, m, kv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,kv", [(3, 3), (4, 40), (40, 70), (70, 70), (3, 900)])
+def test_attention_infinite_scores_gpu(gpu_rt, m, kv):
+    _check_infinite_scores(True, m, kv)
 
 
 def _hints_are_only_hints(dev):
@@ -551,7 +625,8 @@ def test_attention_refuses(fake_rt):
                 dict(block_table=torch.zeros(1, 2, dtype=I32)), dict(block_table=torch.zeros(2, 0, dtype=I32)),
                 dict(out=torch.zeros(3, hq * hd)), dict(out=torch.zeros(2, hq * hd, dtype=dt)),
                 dict(out=torch.zeros(hq * hd, 3, dtype=dt).t()),
-                dict(kv_lens=torch.zeros(2, dtype=I32, device="meta"))):
+                dict(kv_lens=torch.zeros(2, dtype=I32, device="meta")), dict(scale=0.0), dict(scale=math.inf),
+                dict(scale=math.nan)):
         with pytest.raises(ValueError):
             paged.attention(**{**ok, **bad})
 
