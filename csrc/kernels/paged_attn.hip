@@ -166,18 +166,33 @@ __device__ __forceinline__ Request request_of(const PagedAttnArgs& a, uint32_t b
   return r;
 }
 
-// Keys of one split: whole tiles of 64 (two blocks of the few-row body), so that no
-// tile reaches into the next split's keys; at least kMinSplit, so that short
-// requests use few of the launch's splits.
-constexpr int32_t kManyKeys = 64;   // keys of a K / V tile of the many-row body
+// Keys of a K / V tile of the many-row body: 16 KB of K and 16 KB of V. (64 keys of
+// 64 dims: a barrier, a maximum and the addresses of half the work each.)
+template <int HD>
+constexpr int32_t kManyKeys = 8192 / HD;
+
+// Keys of one split: whole tiles of the many-row body (they are whole blocks of
+// the few-row body), so that no tile reaches into the next split's keys; at least
+// kMinSplit, so that short requests use few of the launch's splits.
 constexpr int32_t kMinSplit = 256;
+template <int HD>
 __device__ __forceinline__ int32_t split_keys(int32_t kv, uint32_t splits) {
   const int32_t per = (int32_t)(((uint32_t)kv + splits - 1) / splits);
-  return max((per + kManyKeys - 1) & ~(kManyKeys - 1), kMinSplit);
+  return max((per + kManyKeys<HD> - 1) & ~(kManyKeys<HD> - 1), kMinSplit);
 }
 __device__ __forceinline__ int32_t splits_used(int32_t kv, int32_t per) { return max((kv + per - 1) / per, 1); }
 
 // ---------------------------------------------------------------- few rows
+
+// What the waves of a workgroup leave for each other, behind their blocks in LDS.
+template <int HD, int NB, int NW>
+struct FewJoin {
+  float wm[NW][16 * NB], wl[NW][16 * NB];
+  int32_t first_key[NW][3 * HD];  // take_special; set only by a wave that met one
+  uint32_t special[NW];
+};
+template <int HD, int NB, int NW>
+constexpr uint32_t kFewLds = NW * 32 * kKVRow<HD> * 2 + sizeof(FewJoin<HD, NB, NW>);  // bytes
 
 template <typename T, int HD, int NB, int NW>
 __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, uint32_t b, uint32_t kvh, uint32_t split) {
@@ -191,7 +206,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
   if (rows == 0 || rows > (int32_t)a.plan.few_rows) return;
   const bool looped = rows > R;  // more rows than the host's bound: tile after tile, unsplit
   const int32_t kv = rq.kv > rq.cap ? 0 : rq.kv;
-  const int32_t per = looped ? max(kv, 1) : split_keys(kv, a.plan.few_splits);
+  const int32_t per = looped ? max(kv, 1) : split_keys<HD>(kv, a.plan.few_splits);
   const int32_t used = looped ? 1 : splits_used(kv, per);
   if ((int32_t)split >= used) return;
   const int32_t c0 = (int32_t)split * per, c1 = min(c0 + per, kv);
@@ -200,9 +215,11 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
   uint16_t* vw = lds + wave * (32 * kKVRow<HD>) + 32 * kKRow<HD> + (lane / (HD / 8)) * kVRow<HD> + (lane % (HD / 8)) * 8;
   const uint16_t* kread = lds + wave * (32 * kKVRow<HD>) + col * kKRow<HD> + 8 * quad;
   const uint16_t* vread = lds + wave * (32 * kKVRow<HD>) + 32 * kKRow<HD> + (4 * quad + (col >> 2)) * kVRow<HD> + 4 * (col & 3);
-  __shared__ float wm[NW][R], wl[NW][R];
-  __shared__ int32_t first_key[NW][3 * HD];  // take_special; set only by a wave that met one
-  __shared__ uint32_t special_s[NW];
+  FewJoin<HD, NB, NW>& join = *reinterpret_cast<FewJoin<HD, NB, NW>*>(lds + NW * 32 * kKVRow<HD>);
+  auto& wm = join.wm;
+  auto& wl = join.wl;
+  auto& first_key = join.first_key;
+  auto& special_s = join.special;
   const uint16_t* kbase = a.pages + kvh * a.head_stride;
   const int32_t* table = a.table + b * a.table_ld;
   const float c = a.scale * 1.44269504088896340736f;  // scores in powers of two
@@ -521,12 +538,17 @@ constexpr float kLazy = 6.f;
 // 64 rows a wave (half the LDS reads, one wave per SIMD: 675 us); 32-key steps
 // with the next scores beside the exponentials (444).
 
+template <int HD>
+constexpr uint32_t kManyLds = 2 * kManyKeys<HD> * kKVRow<HD> * 2 + (3 * HD + 1) * 4;  // bytes
+
 template <typename T, int HD>
 __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds, uint32_t x, uint32_t kvh, uint32_t split) {
   constexpr int KS = HD / 16, DT = HD / 32;        // k steps, 32-dim tiles
-  constexpr int LJ = kManyKeys * HD / 8 / 256;     // 16-byte loads of a thread per tile and tensor
-  constexpr uint32_t kTile = kManyKeys * kKVRow<HD>;  // LDS elements of a K and V tile
-  constexpr uint32_t kV = kManyKeys * kKRow<HD>;      // where its V begins
+  constexpr int KT = kManyKeys<HD>, NT = KT / 32;  // keys and 32-key scores of a tile
+  constexpr int LJ = KT * HD / 8 / 256;            // 16-byte loads of a thread per tile and tensor
+  constexpr int kWindow = 1024 / KT;               // tiles whose groups of 16 keys fill a wave's lanes
+  constexpr uint32_t kTile = KT * kKVRow<HD>;         // LDS elements of a K and V tile
+  constexpr uint32_t kV = KT * kKRow<HD>;             // where its V begins
   const uint32_t lane = threadIdx.x & 63, wave = wave_id(), tid = threadIdx.x;
   const uint32_t col = lane & 31, half = lane >> 5;
   const uint32_t g = a.hq / a.hkv;
@@ -539,7 +561,7 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
   // keys that any row of the tile sees, and this split's share
   const int32_t last = rq.kv - rq.n + (min(r0 + kManyRows, rows) - 1) / (int32_t)g;
   const int32_t kend = bad ? 0 : max(last + 1, 0);
-  const int32_t per = split_keys(kend, a.plan.many_splits), used = splits_used(kend, per);
+  const int32_t per = split_keys<HD>(kend, a.plan.many_splits), used = splits_used(kend, per);
   if ((int32_t)split >= used) return;
   const int32_t c0 = (int32_t)split * per, c1 = min(c0 + per, kend);
   const uint16_t* kbase = a.pages + kvh * a.head_stride;
@@ -581,16 +603,16 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
   const uint32_t vread = kV + (4 * half + ((lane & 15) >> 2)) * kVRow<HD> + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const uint32_t mine = (tid / (HD / 8)) % 16 * HD + tid % (HD / 8) * 8;  // in its group of 16 keys
 
-  // Where the lane's group of 16 keys (one page) begins, for 16 tiles. A group
+  // Where the lane's group of 16 keys (one page) begins, for kWindow tiles. A group
   // whose page is outside the pool reads page 0; the first such key makes the
   // rows that see it NaN.
   int32_t first_missing = rq.kv > rq.cap ? 0 : kNever;
   uint32_t at_lo = 0, at_hi = 0;
   auto find_groups = [&](int32_t i) {
-    const int32_t t = c0 + i * kManyKeys + 16 * (int32_t)lane;
+    const int32_t t = c0 + i * KT + 16 * (int32_t)lane;
     int32_t page = t < c1 ? table[t >> a.page_shift] : 0;
     const uint64_t outside = __ballot((uint32_t)page >= a.num_pages);
-    if (outside) first_missing = min(first_missing, c0 + i * kManyKeys + 16 * (int32_t)__builtin_ctzll(outside));
+    if (outside) first_missing = min(first_missing, c0 + i * KT + 16 * (int32_t)__builtin_ctzll(outside));
     if ((uint32_t)page >= a.num_pages) page = 0;
     const uint64_t at = (uint64_t)page * a.page_stride + (uint64_t)((uint32_t)t & ((1u << a.page_shift) - 1u)) * HD;
     at_lo = (uint32_t)at;
@@ -598,28 +620,28 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
   };
   u32x4 kr[LJ], vr[LJ];
   auto load = [&](int32_t i) {
-    if ((i & 15) == 0) find_groups(i);
+    if (i % kWindow == 0) find_groups(i);
 #pragma unroll
     for (int j = 0; j < LJ; ++j) {
-      const uint32_t grp = 4 * (i & 15) + (j * 256 + wave * 64) / (HD / 8) / 16;  // wave-uniform
+      const uint32_t grp = KT / 16 * (i % kWindow) + (j * 256 + wave * 64) / (HD / 8) / 16;  // wave-uniform
       const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_lo, grp) |
                           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_hi, grp) << 32;
       kr[j] = *reinterpret_cast<const u32x4*>(kbase + at + mine);
       vr[j] = *reinterpret_cast<const u32x4*>(kbase + a.kv_stride + at + mine);
     }
   };
-  const int32_t tiles = (c1 - c0 + kManyKeys - 1) / kManyKeys;
+  const int32_t tiles = (c1 - c0 + KT - 1) / KT;
   const int32_t first = rq.kv - rq.n + r0 / (int32_t)g;  // of the whole tile of rows
-  __shared__ int32_t first_key[3 * HD];  // take_special
-  __shared__ uint32_t special_s;
+  int32_t* first_key = reinterpret_cast<int32_t*>(lds + 2 * kTile);  // [3 * HD], take_special
+  int32_t& special_s = first_key[3 * HD];
   for (uint32_t e = tid; e < 3 * HD; e += 256) first_key[e] = kNever;
   if (tid == 0) special_s = 0;
   if (tiles > 0) load(0);
   __syncthreads();
   for (int32_t i = 0; i < tiles; ++i) {
-    const int32_t t0 = c0 + i * kManyKeys;
+    const int32_t t0 = c0 + i * KT;
     uint16_t* buf = lds + (i & 1) * kTile;
-    const bool tile_masked = t0 + kManyKeys - 1 > first;
+    const bool tile_masked = t0 + KT - 1 > first;
     bool odd = false;
     if (tile_masked) {
 #pragma unroll
@@ -645,9 +667,9 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
     // Between the barrier and the last product a wave goes before those that load
     // and store (430 -> 421 us for the 4096 rows, 52 -> 49 for 12 x 400 64-wide).
     __builtin_amdgcn_s_setprio(1);
-    f32x16_t s[2];
+    f32x16_t s[NT];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
 #pragma unroll
@@ -657,22 +679,24 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
     // six operands ahead of the products: an LDS read takes longer than one
     __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
-    for (int k = 0; k < 2 * KS - 6; ++k) {
+    for (int k = 0; k < NT * KS - 6; ++k) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     // register e of s[t] is key 32 t + 8 (e / 4) + 4 half + e % 4
-    if (t0 + kManyKeys - 1 > wfirst) {
+    if (t0 + KT - 1 > wfirst) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (t0 + 32 * t + 8 * (e / 4) + 4 * (int32_t)half + e % 4 > pos) s[t][e] = -__builtin_inff();
     }
-    float mx = max2(s[0][0], s[1][0]);
+    float mx = -__builtin_inff();
 #pragma unroll
-    for (int e = 1; e < 16; ++e) mx = max2(max2(mx, s[0][e]), s[1][e]);
+    for (int t = 0; t < NT; t += 2)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = max2(max2(mx, s[t][e]), s[t + 1][e]);
     mx = max_other_half(mx) * c;
     if (__any(mx > m + kLazy) || i == 0) {
       const float mn = max2(m, mx);
@@ -709,8 +733,8 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
     p[0] = exponentials(0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      if (kt < 3) {
+    for (int kt = 0; kt < 2 * NT; ++kt) {
+      if (kt + 1 < 2 * NT) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) va[(kt + 1) & 1][d] = v_frag(d, kt + 1);
         p[(kt + 1) & 1] = exponentials(kt + 1);
@@ -766,7 +790,7 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
 
 template <typename T, int HD, int NB, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) k_paged_few(PagedAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[NW * 32 * kKVRow<HD>];
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kFewLds<HD, NB, NW> / 2];
   few_body<T, HD, NB, NW>(a, lds, blockIdx.z, blockIdx.x, blockIdx.y);
 }
 
@@ -774,7 +798,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_paged_few(PagedAttnArgs a) {
 // requests, which fill in beside them.
 template <typename T, int HD, int NB>
 __global__ void __launch_bounds__(256, 2) k_paged_mixed(PagedAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kManyKeys * kKVRow<HD>];
+  __shared__ __attribute__((aligned(16))) uint16_t lds[std::max(kFewLds<HD, NB, 4>, kManyLds<HD>) / 2];  // 2 fit a CU
   uint32_t i = blockIdx.x;
   const uint32_t kvh = i % a.hkv;  // a head's workgroups share their K and V, and with 8 heads an XCD's L2
   i /= a.hkv;
@@ -828,7 +852,7 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttnArgs a) {
     at = ((uint64_t)b * a.hkv + kvh) * splits * R;
   }
   if (rq.kv > rq.cap) return;
-  const int32_t used = splits_used(keys, split_keys(keys, splits));
+  const int32_t used = splits_used(keys, split_keys<HD>(keys, splits));
   if (used == 1) return;
   const int32_t rows = rq.n * (int32_t)g;
 #pragma unroll

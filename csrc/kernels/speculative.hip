@@ -91,10 +91,21 @@ __device__ __forceinline__ void weights(const VerifyRow<T>& r, uint32_t i0, uint
   const T* qr = r.q && !whole ? r.q : r.p;
   const bool no_q = whole || !r.q;
   T p[N], q[N];
+  constexpr uint32_t E = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(E)));
+  if (step == 1 && i0 + N <= V && (((uintptr_t)(r.p + i0) | (uintptr_t)(qr + i0)) & 15) == 0) {
+    // consecutive entries: 16 bytes a load, or the lanes' 64-byte stride costs a
+    // cache line for each of them
 #pragma unroll
-  for (uint32_t k = 0; k < N; ++k) p[k] = r.p[min(i0 + k * step, V - 1)];
+    for (uint32_t k = 0; k < N; k += E) *reinterpret_cast<vec*>(p + k) = *reinterpret_cast<const vec*>(r.p + i0 + k);
 #pragma unroll
-  for (uint32_t k = 0; k < N; ++k) q[k] = qr[min(i0 + k * step, V - 1)];
+    for (uint32_t k = 0; k < N; k += E) *reinterpret_cast<vec*>(q + k) = *reinterpret_cast<const vec*>(qr + i0 + k);
+  } else {
+#pragma unroll
+    for (uint32_t k = 0; k < N; ++k) p[k] = r.p[min(i0 + k * step, V - 1)];
+#pragma unroll
+    for (uint32_t k = 0; k < N; ++k) q[k] = qr[min(i0 + k * step, V - 1)];
+  }
 #pragma unroll
   for (uint32_t k = 0; k < N; ++k) {
     const uint32_t i = i0 + k * step;
@@ -133,6 +144,16 @@ __device__ __forceinline__ double quarter_sum(const VerifyRow<T>& r, uint32_t i0
   return wave_sum_f64(sum);
 }
 
+// Sum of this lane's value and the lower lanes'.
+__device__ __forceinline__ double wave_scan_f64(double x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) x += y;
+  }
+  return x;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) k_verify_sums(VerifyArgs a) {
   __shared__ double part[4];
@@ -168,9 +189,13 @@ __global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a) {
     pick_s = INT32_MAX;
     last_s = -1;
   }
-  double total = sum0;
-  for (uint32_t c = 64 + lane; c < nchunks; c += 64) total += sums[c];
-  total = wave_sum_f64(total);
+  const double upto0 = wave_scan_f64(sum0);
+  double total = __shfl(upto0, 63, 64);
+  if (nchunks > 64) {
+    double rest = 0.0;
+    for (uint32_t c = 64 + lane; c < nchunks; c += 64) rest += sums[c];
+    total += wave_sum_f64(rest);
+  }
   // Nothing remains of the target: its own row, walked by this workgroup alone,
   // once for the sum and once for the entry.
   const bool whole = !(total > 0.0);
@@ -182,13 +207,7 @@ __global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a) {
     double run = 0.0;
     for (uint32_t c0 = 0; c0 < nchunks; c0 += 64) {
       const double own = c0 == 0 ? sum0 : c0 + lane < nchunks ? sums[c0 + lane] : 0.0;
-      double x = own;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(x, o, 64);
-        if ((int)lane >= o) x += y;
-      }
-      const double to = run + x;
+      const double to = c0 == 0 ? upto0 : run + wave_scan_f64(own);
       const uint64_t past = __ballot(own > 0.0 && to > aim), some = __ballot(own > 0.0);
       if (some) {
         const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
@@ -209,12 +228,7 @@ __global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a) {
       weights<T>(r, i0, 1, a.V, whole, w);
 #pragma unroll
       for (uint32_t k = 0; k < kOwn; ++k) mine += w[k];
-      double x = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(x, o, 64);
-        if ((int)lane >= o) x += y;
-      }
+      const double x = wave_scan_f64(mine);
       __syncthreads();  // pick_s is set, and the chunk before is done with `part`
       if (lane == 63) part[wave] = x;
       __syncthreads();
