@@ -23,16 +23,28 @@ static inline uint16_t f2bf(float f) {
   u += 0x7FFFu + ((u >> 16) & 1u);
   return (uint16_t)(u >> 16);
 }
+// fp16 by hand: not every host compiler that builds this file has the type.
 static inline float h2f(uint16_t b) {
-  _Float16 h;
-  memcpy(&h, &b, 2);
-  return (float)h;
+  const uint32_t sign = (uint32_t)(b & 0x8000u) << 16, rest = b & 0x7FFFu;
+  if (rest < 0x400u) {  // zero, subnormal
+    const float f = (float)rest * 0x1p-24f;
+    return sign ? -f : f;
+  }
+  const uint32_t u = sign | (rest >= 0x7C00u ? 0x7F800000u | (rest & 0x3FFu) << 13 : (rest << 13) + (112u << 23));
+  float f;
+  memcpy(&f, &u, 4);
+  return f;
 }
-static inline uint16_t f2h(float f) {
-  const _Float16 h = (_Float16)f;
-  uint16_t b;
-  memcpy(&b, &h, 2);
-  return b;
+static inline uint16_t f2h(float f) {  // to nearest, ties to even
+  uint32_t u;
+  memcpy(&u, &f, 4);
+  const uint16_t sign = (uint16_t)((u >> 16) & 0x8000u);
+  u &= 0x7FFFFFFFu;
+  if (u > 0x7F800000u) return (uint16_t)(sign | 0x7E00u | ((u >> 13) & 0x3FFu));
+  if (u >= 0x477FF000u) return (uint16_t)(sign | 0x7C00u);  // 65520 and above
+  if (u < 0x38800000u) return (uint16_t)(sign | (uint32_t)std::nearbyint(std::fabs(f) * 0x1p24f));  // below 2^-14
+  u += 0xFFFu + ((u >> 13) & 1u);
+  return (uint16_t)(sign | ((u - (112u << 23)) >> 13));
 }
 static inline float load16(uint16_t b, uint32_t elem) { return elem == ELEM_F16 ? h2f(b) : bf2f(b); }
 static inline uint16_t store16(float f, uint32_t elem) { return elem == ELEM_F16 ? f2h(f) : f2bf(f); }
