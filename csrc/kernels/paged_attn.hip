@@ -18,12 +18,14 @@
 // K and V rows go global -> registers -> LDS (the next tile's loads fly while
 // this one is multiplied).
 //
-// Two bodies. `few` (up to 16 NB rows per kv head: single tokens, drafts) is
-// bound by the KV bytes: each wave streams its own 32-key blocks through
-// wave-private LDS without barriers, the waves join at the end. `many` (prompt
-// chunks) is bound by the matrix cores: four waves of 32 rows share each
-// 64-key tile. One launch serves both kinds in a mixed batch. The key axis is
-// split where rows are few; k_paged_combine joins the parts.
+// Two bodies. `few` (up to 32 rows per kv head: single tokens, drafts) is bound
+// by the KV bytes: each wave streams its own 32-key blocks through wave-private
+// LDS without barriers, the waves join at the end. 64 tokens of 64 query and 8 kv
+// heads at up to 2048 keys: 69 us; 4 tokens of 32 / 8 heads at up to 131071: 258
+// us, 5.6 TB/s of K and V. `many` (prompt chunks) is bound by the matrix cores:
+// four waves of 32 rows share each tile of 64 keys (128 of 64 dims). One launch
+// serves both kinds in a mixed batch. The key axis is split where rows are few;
+// k_paged_combine joins the parts.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -528,10 +530,10 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, uint32_t x, ui
 // after the first tiles. fp16: 2^(kLazy + shift) stays below 65504.
 constexpr float kLazy = 6.f;
 
-// A wave owns 32 rows, the workgroup walks tiles of 64 keys in two LDS buffers:
-// tile i + 1 flies into registers while tile i is multiplied, one barrier a tile
+// A wave owns 32 rows, the workgroup walks tiles of 8192 / HD keys in two LDS
+// buffers: tile i + 1 flies into registers while tile i is multiplied, one barrier a tile
 // (a buffer is written two tiles after it was read). 4096 rows behind 4095 cached
-// keys of the 8B heads: 417 us, 990 TFLOP/s, where the library's 8192^3 product
+// keys of the 8B heads: 413 us, 1000 TFLOP/s, where the library's 8192^3 product
 // of such values reaches 1140 - 1230 on this card. The wave alternates between
 // the matrix cores (1024 cycles a tile) and the vector ALU (1000, half of it
 // exponentials); two workgroups a CU overlap them in part. Tried and not kept:

@@ -84,10 +84,8 @@ def _check_pool(op: str, dtype, shape, stride, rows_dtype) -> None:
         raise ValueError(f"{op}: {rows_dtype} rows over {dtype} pages")
 
 
-def _aligned(op: str, *pointers: int) -> None:
-    for p in pointers:
-        if p % 16:
-            raise ValueError(f"{op}: tensors must be 16-byte aligned")
+def _unaligned(op: str):
+    raise ValueError(f"{op}: tensors must be 16-byte aligned")
 
 
 class Plan(NamedTuple):
@@ -150,7 +148,7 @@ def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pages: torc
     hd / 2] (rotate-half). A row with position -1 is padding: its q is 0 and
     nothing is stored, as for a slot outside the pool; a position behind the
     tables gives NaN. Slots of one call are distinct (of two rows with one slot
-    either's values may stay)."""
+    either's values may stay); the pool's pages share no memory."""
     n, hd, num, size, max_pos = _rope_layout(qkv.dtype, qkv.shape, qkv.stride(), pages.dtype, pages.shape,
                                              pages.stride(), cos.dtype, cos.shape, cos.stride(), sin.dtype, sin.shape,
                                              sin.stride(), hq, hkv)
@@ -160,7 +158,8 @@ def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pages: torc
     dev, stream = _where("rope_kv", qkv, cos, sin, pages, positions, slots)
     q = qkv.new_empty((n, hq, hd))
     x, c, s, p = qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), pages.data_ptr()
-    _aligned("rope_kv", x, c, s, p)
+    if (x | c | s | p) & 15:
+        _unaligned("rope_kv")
     kv_stride, page_stride, head_stride = pages.stride()[:3]
     lib.paged_rope(dev, stream, x, qkv.stride(0), c, s, positions.data_ptr(), slots.data_ptr(), q.data_ptr(), p,
                    kv_stride, page_stride, head_stride, n, hq, hkv, hd, num, size, max_pos, _ELEM[qkv.dtype])
@@ -172,6 +171,11 @@ def _rope_layout(dtype, qkv, qkv_stride, pool_dtype, pool, pool_stride, cos_dtyp
                  sin_stride, hq, hkv):
     _check_pool("rope_kv", pool_dtype, pool, pool_stride, dtype)
     _, num, heads, size, hd = pool
+    span = 0  # an element of one page may not be an element of another: the rows are written
+    for st, n in sorted((st, n) for n, st in zip(pool[:4], pool_stride[:4]) if n > 1):
+        if st < max(span, hd):
+            raise ValueError("rope_kv: the pool's pages overlap")
+        span = st * (n - 1) + max(span, hd)
     if hkv != heads or hq < 1 or hd % 16:
         raise ValueError(f"rope_kv: {hkv} kv heads over a pool of {heads}, hd {hd} (a multiple of 16)")
     if len(qkv) != 2 or qkv[1] != (hq + 2 * hkv) * hd or qkv_stride[1] != 1 or (qkv[0] > 1 and qkv_stride[0] % 8):
@@ -194,7 +198,8 @@ def attention(q: torch.Tensor, pages: torch.Tensor, cu_q: torch.Tensor, kv_lens:
     need a page outside the pool or beyond their table row give NaN.
 
     ``max_q`` / ``max_kv``: the host's bounds of rows and length per request; they
-    only choose how the work is split (default: n and the table's width)."""
+    only choose how the work is split (default: n and the table's width). ``out``
+    shares no memory with q or the pool. Limits: 65535 requests, 2^30 tokens each."""
     n, B, hq, hkv, hd, num, size, width = _attention_layout(
         q.dtype, q.shape, q.stride(), pages.dtype, pages.shape, pages.stride(), kv_lens.shape, block_table.dtype,
         block_table.shape, block_table.stride())
@@ -215,10 +220,11 @@ def attention(q: torch.Tensor, pages: torch.Tensor, cu_q: torch.Tensor, kv_lens:
     if dev >= 0:
         part_bytes = lib.paged_attn_workspace(n, B, hq, hkv, hd, max_q, max_kv)
         if part_bytes:
-            work = torch.empty(part_bytes, dtype=torch.uint8, device=q.device)
+            work = q.new_empty(part_bytes // 2)
             part = work.data_ptr()
     x, p, y = q.data_ptr(), pages.data_ptr(), out.data_ptr()
-    _aligned("attention", x, p, y)
+    if (x | p | y) & 15:
+        _unaligned("attention")
     q_stride, q_head_stride, _ = q.stride()
     kv_stride, page_stride, head_stride = pages.stride()[:3]
     lib.paged_attn(dev, stream, x, q_stride, q_head_stride, p, kv_stride, page_stride, head_stride, cu_q.data_ptr(),

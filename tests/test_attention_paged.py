@@ -220,6 +220,23 @@ def test_rope_kv_gpu(gpu_rt, dt, n, hq, hkv, hd, P, layout, pad):
     _check_rope(True, dt, n, hq, hkv, hd, P, layout, pad)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_rope_kv_rounds_as_torch_cpu(fake_rt, dt):
+    """Every 16-bit value times a cosine (sine 0, so one f32 product rounded once)."""
+    hd, P = 64, 16
+    x = torch.arange(-2**15, 2**15, dtype=torch.int32).to(torch.int16).view(dt).view(-1, 1, hd // 2)
+    n, pages = x.shape[0], torch.zeros(2, 1, 1, P, hd, dtype=dt)
+    zero = torch.zeros_like(x)
+    for c in (1.0, 0.3712, 2.0 ** -9, 2.0 ** -20, 1.7):
+        cos, sin = torch.full((1, hd // 2), c), torch.zeros(1, hd // 2)
+        q = paged.rope_kv(torch.cat([x, zero, x, zero, x, zero], 2).view(n, 3 * hd), cos, sin, pages,
+                          torch.zeros(n, dtype=I32), torch.full((n,), -1, dtype=I32), 1, 1)
+        want = (x.float() * cos).to(dt)
+        got = q[:, :, :hd // 2]
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got[~want.isnan()].view(torch.int16), want[~want.isnan()].view(torch.int16)), c
+
+
 @pytest.mark.gpu
 def test_rope_kv_no_rows_gpu(gpu_rt):
     _check_rope(True, torch.bfloat16, 0, 8, 2, 128, 16)
@@ -242,6 +259,22 @@ def test_rope_kv_refuses(fake_rt):
                 dict(slots=torch.zeros(3, dtype=I32, device="meta"))):
         with pytest.raises(ValueError):
             paged.rope_kv(**{**ok, **bad})
+
+
+def test_rope_kv_refuses_overlapping_pages(fake_rt):
+    """A pool whose pages share memory is refused where it is written; slices and
+    permutations of a larger one are not."""
+    n, hq, hkv, hd, P = 2, 2, 2, 64, 16
+    ok = dict(qkv=torch.zeros(n, (hq + 2 * hkv) * hd, dtype=torch.bfloat16), cos=torch.zeros(8, hd // 2),
+              sin=torch.zeros(8, hd // 2), positions=_i32([0, 1], "cpu"), slots=_i32([0, 1], "cpu"), hq=hq, hkv=hkv)
+    flat = torch.zeros(2 * 4 * hkv * P * hd, dtype=torch.bfloat16)
+    rows, head, page = P * hd, P * hd, hkv * P * hd
+    for kv_s, page_s, head_s in ((4 * page, page, head), (page, 2 * page, head), (rows, 2 * page, 2 * rows)):
+        paged.rope_kv(pages=flat.as_strided((2, 2, hkv, P, hd), (kv_s, page_s, head_s, hd, 1)), **ok)
+    for kv_s, page_s, head_s in ((0, page, head), (4 * page, 0, head), (4 * page, page, 0), (page, page, head),
+                                 (4 * page, page - 8, head), (4 * page, page, head - hd)):
+        with pytest.raises(ValueError):
+            paged.rope_kv(pages=flat.as_strided((2, 2, hkv, P, hd), (kv_s, page_s, head_s, hd, 1)), **ok)
 
 
 # ---------------------------------------------------------------- attention
