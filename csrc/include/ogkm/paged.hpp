@@ -53,6 +53,7 @@ struct PagedRopeArgs {
 // How a call's work is laid out: from the host's bounds alone, so that one layout
 // serves every content of the device's lengths.
 struct PagedAttnPlan {
+  uint32_t most_rows;   // rows of a request per kv head, by the host's bound
   uint32_t few_rows;    // requests of up to so many rows per kv head take the `few` body
   uint32_t few_blocks;  // its column blocks of 16 rows: 1 or 2
   uint32_t few_waves;   // waves of a workgroup: 4 or 8

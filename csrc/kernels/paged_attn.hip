@@ -151,6 +151,12 @@ __device__ __forceinline__ float max_other_half(float x) {  // of lanes l and l 
   return max2(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
 }
 
+// What a sum over the maximum m counts for over the maximum mx >= m; a sum that
+// saw only -inf (0 or NaN) keeps its value where nothing else is there.
+__device__ __forceinline__ float scale_to(float m, float mx) {
+  return m == mx ? 1.f : m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+}
+
 // The wave's number, known to the compiler as uniform: bounds, page ids and
 // addresses that follow from it stay in scalar registers.
 __device__ __forceinline__ uint32_t wave_id() { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
@@ -813,26 +819,38 @@ __global__ void __launch_bounds__(256, 2) k_paged_mixed(PagedAttnArgs a) {
   }
 }
 
-// Joins the splits: a thread adds four dims of kJoin rows over the splits, with a
-// running maximum, four splits' loads in flight. A workgroup takes a part of one
-// unit - a tile of many rows, or the rows of a request of few - and the units'
-// first blocks are those of the tiles.
-constexpr uint32_t kJoin = 4;
-template <int HD>
-constexpr uint32_t join_parts(uint32_t rows) { return (rows * (HD / 4) + 256 * kJoin - 1) / (256 * kJoin); }
+// Joins the splits. A unit is a tile of many rows, or the rows of a request of
+// few; the units' first workgroups are those of the tiles. A thread takes four
+// dims of a row and a slice of the splits (at most kSlices), four splits' loads in
+// flight, with a running maximum; the slices meet in LDS.
+constexpr uint32_t kSlices = 16;
+__host__ __device__ constexpr uint32_t join_slices(uint32_t splits) {
+  uint32_t z = 1;
+  while (z < kSlices && 4 * z < splits) z *= 2;
+  return z;
+}
+// Workgroups of a unit of `rows` rows (the host's bound; what lies beyond it is
+// taken in further rounds): one round, but no more than 2048 workgroups in all.
+uint32_t join_parts(uint64_t rows, uint32_t hd, uint32_t splits, uint64_t units) {
+  const uint64_t all = (rows * (hd / 4) * join_slices(splits) + 255) / 256;
+  return (uint32_t)std::max<uint64_t>(std::min<uint64_t>(all, 2048 / std::max<uint64_t>(units, 1)), 1);
+}
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_paged_combine(PagedAttnArgs a) {
+__global__ void __launch_bounds__(256) k_paged_combine(PagedAttnArgs a, uint32_t many_parts, uint32_t few_parts) {
+  __shared__ f32x4_t slice_o[256];
+  __shared__ float slice_m[256], slice_l[256];
   const uint32_t kvh = blockIdx.y;
   const uint32_t g = a.hq / a.hkv;
-  const uint32_t many_blocks = a.plan.many_splits > 1 ? a.plan.many_tiles * join_parts<HD>(kManyRows) : 0;
-  uint32_t b, splits, R, part;
+  const uint32_t many_blocks = a.plan.many_splits > 1 ? a.plan.many_tiles * many_parts : 0;
+  uint32_t b, splits, R, part, parts;
   int32_t r0, keys;  // first row of the unit in its request, keys that were split
   uint64_t at;
   Request rq;
   if (blockIdx.x < many_blocks) {
-    const uint32_t x = blockIdx.x / join_parts<HD>(kManyRows);
-    part = blockIdx.x % join_parts<HD>(kManyRows);
+    parts = many_parts;
+    const uint32_t x = blockIdx.x / parts;
+    part = blockIdx.x % parts;
     int32_t ti;
     if (!find_tile(a, x, &b, &ti)) return;
     rq = request_of(a, b);
@@ -844,53 +862,75 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttnArgs a) {
   } else {
     const uint32_t i = blockIdx.x - many_blocks;
     R = 16 * a.plan.few_blocks;
-    b = i / join_parts<HD>(R);
-    part = i % join_parts<HD>(R);
+    splits = a.plan.few_splits;
+    parts = few_parts;
+    b = i / parts;
+    part = i % parts;
     rq = request_of(a, b);
     if (rq.n * (int32_t)g > (int32_t)R) return;
     r0 = 0;
     keys = rq.kv;
-    splits = a.plan.few_splits;
     at = ((uint64_t)b * a.hkv + kvh) * splits * R;
   }
   if (rq.kv > rq.cap) return;
   const int32_t used = splits_used(keys, split_keys<HD>(keys, splits));
   if (used == 1) return;
-  const int32_t rows = rq.n * (int32_t)g;
-#pragma unroll
-  for (uint32_t u = 0; u < kJoin; ++u) {
-    const uint32_t item = (part * kJoin + u) * 256 + threadIdx.x, rr = item / (HD / 4), d = item % (HD / 4) * 4;
-    const int32_t r = r0 + (int32_t)rr;
-    if (rr >= R || r >= rows) continue;
+  const uint32_t items = min((uint32_t)(rq.n * (int32_t)g - r0), R) * (HD / 4);
+  const uint32_t slices = join_slices(splits), per = 256 / slices;
+  const uint32_t slice = threadIdx.x / per, own = threadIdx.x % per;
+  for (uint32_t first = part * per; first < items; first += parts * per) {
+    const uint32_t item = first + own, rr = item / (HD / 4), d = item % (HD / 4) * 4;
+    const bool in = item < items;
     float big = -__builtin_inff(), sum = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int32_t s = 0; s < used; s += 4) {
-      float m[4], l[4];
-      f32x4_t x[4];
+    if (in) {
+      for (uint32_t s = slice; s < (uint32_t)used; s += 4 * slices) {
+        float m[4], l[4];
+        f32x4_t x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint64_t i = at + rr + (uint64_t)min(s + e, used - 1) * R;
-        m[e] = a.part_ml[2 * i];
-        l[e] = a.part_ml[2 * i + 1];
-        x[e] = *reinterpret_cast<const f32x4_t*>(a.part_o + i * HD + d);
+        for (int e = 0; e < 4; ++e) {
+          const uint64_t i = at + rr + (uint64_t)min(s + e * slices, (uint32_t)used - 1) * R;
+          m[e] = a.part_ml[2 * i];
+          l[e] = a.part_ml[2 * i + 1];
+          x[e] = *reinterpret_cast<const f32x4_t*>(a.part_o + i * HD + d);
+        }
+        float mx = big;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = max2(mx, m[e]);
+        const float old = scale_to(big, mx);
+        sum *= old;
+        o *= old;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (s + e * slices < (uint32_t)used) {
+            const float f = scale_to(m[e], mx);
+            sum += f * l[e];
+            o += f * x[e];
+          }
+        big = mx;
       }
-      float mx = big;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx = max2(mx, m[e]);
-      const float old = big == mx ? 1.f : big == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(big - mx);
-      sum *= old;
-      o *= old;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float f = s + e >= used ? 0.f : m[e] == mx ? 1.f : m[e] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[e] - mx);
-        if (s + e < used) {
-          sum += f * l[e];
-          o += f * x[e];
+    }
+    if (slices > 1) {
+      __syncthreads();  // the slices of the round before are read
+      slice_o[threadIdx.x] = o;
+      slice_m[threadIdx.x] = big;
+      slice_l[threadIdx.x] = sum;
+      __syncthreads();
+      if (slice == 0) {
+        float mx = big;
+        for (uint32_t z = 1; z < slices; ++z) mx = max2(mx, slice_m[z * per + own]);
+        const float f0 = scale_to(big, mx);
+        sum *= f0;
+        o *= f0;
+        for (uint32_t z = 1; z < min(slices, (uint32_t)used); ++z) {
+          const float f = scale_to(slice_m[z * per + own], mx);
+          sum += f * slice_l[z * per + own];
+          o += f * slice_o[z * per + own];
         }
       }
-      big = mx;
     }
-    const uint32_t tok = (uint32_t)r / g, h = (uint32_t)r - tok * g;
+    if (!in || slice) continue;
+    const uint32_t r = (uint32_t)r0 + rr, tok = r / g, h = r - tok * g;
     const float inv = rq.kv - rq.n + (int32_t)tok < 0 ? 0.f : 1.f / sum;
     uint16_t* out = a.out + (uint64_t)(rq.row0 + tok) * a.out_stride + (uint64_t)(kvh * g + h) * HD + d;
     // sum 0: the row saw only scores of -inf, 0 / 0
@@ -913,10 +953,14 @@ hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t s) {
     else
       hipLaunchKernelGGL((k_paged_few<T, HD, NB, 4>), grid, dim3(256), 0, s, a);
   }
-  const uint64_t groups = (p.many_splits > 1 ? (uint64_t)p.many_tiles * join_parts<HD>(kManyRows) : 0) +
-                          (p.few_splits > 1 ? (uint64_t)a.B * join_parts<HD>(16 * NB) : 0);
+  const uint64_t many_units = p.many_splits > 1 ? p.many_tiles : 0, few_units = p.few_splits > 1 ? a.B : 0;
+  const uint64_t units = (many_units + few_units) * a.hkv;
+  const uint32_t many_parts = join_parts(std::min<uint32_t>(p.most_rows, kManyRows), HD, p.many_splits, units);
+  const uint32_t few_parts = join_parts(std::min<uint32_t>(p.most_rows, 16 * NB), HD, p.few_splits, units);
+  const uint64_t groups = many_units * many_parts + few_units * few_parts;
   if (groups >= (1u << 24)) return hipErrorInvalidValue;
-  if (groups) hipLaunchKernelGGL((k_paged_combine<T, HD>), dim3((uint32_t)groups, a.hkv), dim3(256), 0, s, a);
+  if (groups)
+    hipLaunchKernelGGL((k_paged_combine<T, HD>), dim3((uint32_t)groups, a.hkv), dim3(256), 0, s, a, many_parts, few_parts);
   return hipGetLastError();
 }
 
@@ -937,6 +981,7 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
   // 512 registers: 32 x 5 drafted rows of 8 heads at up to 8191 keys took 48 us,
   // the other body's half-empty tiles take 38.)
   const bool only_few = most <= 32;
+  p.most_rows = (uint32_t)most;
   const uint64_t few = only_few ? most : g;  // rows that the few-row body is laid out for
   p.few_blocks = few <= 16 ? 1 : 2;
   p.many_splits = 1;
@@ -946,20 +991,28 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
     // 0 rows where one token already takes more
     p.few_rows = g <= 32 ? 16 * p.few_blocks : 0;
     p.many_tiles = (uint32_t)(n * g / kManyRows + std::min<uint64_t>(B, n * g / (p.few_rows + 1)));
-    // A workgroup a CU; the joining of more splits costs more than they save. us at
-    // 128 / 256 / 512 / 1024 workgroups: 512 rows behind 3584 keys (8B heads) 93 /
-    // 64 / 58 / 72, 1040 behind 1407 (8 heads, one kv head) 41 / 31 / 40 / 41, 15
-    // requests of 419 rows 55 / 53 / 74 / 78, 16 behind 32752 56 / 49 / 69 / 115.
+    // One workgroup a CU; two, those of single tokens among them, where each keeps
+    // 512 keys of 128 dims (fewer do not pay for its start). us at 256 / 512 / 768 workgroups: 32 requests of 5 rows
+    // (8 heads, one kv head) at up to 8191 keys 33 / 31 / 35, 16 of 9 at 16384 43 /
+    // 37 / 35, 512 rows behind 3584 (8B heads) 61 / 54 / 66; but 1040 behind 1407
+    // (8 heads, one kv head) 30 / 41 / 40, 15 requests of 105 rows of 64-wide heads
+    // at 2047 32 / 35 / 35; 511 rows (8B heads) beside 32 single tokens 55 in one
+    // piece, 61 in two.
     const uint64_t wgs = std::max<uint64_t>(p.many_tiles * heads, 1);
-    p.many_splits = (uint32_t)std::min<uint64_t>((256 + wgs - 1) / wgs, key_splits);
+    const uint64_t one = (256 + wgs - 1) / wgs, two = (512 + wgs - 1 - std::min<uint64_t>(B * heads, 512)) / wgs;
+    const uint64_t worth = (uint64_t)max_kv * hd / (512 * 128);
+    p.many_splits = (uint32_t)std::min(std::max(one, std::min(two, worth)), key_splits);
   }
   // A workgroup a CU: four waves with a block each in flight draw what HBM gives.
   // us at 128 / 256 / 512 / 1024 workgroups: 4 requests of up to 131071 keys 343 /
   // 257 / 257 / 257, 16 of 4096 49 / 42 / 44 / 44, 64 of 2048 (70B heads) 70 / 70 /
   // 70 / 78. At least kMinSplit keys each: 128, 256 and 512 are within 2 us, 1024
-  // loses 3 on 4 requests of 8192.
-  const uint64_t wgs = std::max<uint64_t>(B * heads, 1);
-  p.few_splits = (uint32_t)std::min<uint64_t>((256 + wgs - 1) / wgs, key_splits);
+  // loses 3 on 4 requests of 8192. Half of that beside longer requests, whose
+  // tiles fill the CUs too (12 x 511 rows and 36 single tokens of 64-wide heads at
+  // up to 2047 keys: 53 us with two splits and their joining, 49.6 without; a token
+  // each of 4 requests at 131071 and a chunk: 113, and 142 at 64 workgroups).
+  const uint64_t wgs = std::max<uint64_t>(B * heads, 1), few_wgs = only_few ? 256 : 128;
+  p.few_splits = (uint32_t)std::min<uint64_t>((few_wgs + wgs - 1) / wgs, key_splits);
   // Short contexts of few requests: eight waves and no second launch. us with it /
   // with splits: one request of the 8B heads at 512 keys 9.4 / 11.8, at 1025 12.4 /
   // 11.8, at 1536 15.1 / 11.6; 4 requests of 64-wide heads at 1025 8.9 / 11.6.

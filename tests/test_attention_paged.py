@@ -338,7 +338,7 @@ def _check_attn(gpu, dt, ql, kl, hq, hkv, hd, P, layout="contiguous", pad=0, hin
         for t in range(k):
             pool[:, table[b, t // P], :, t % P] = torch.randn(2, hkv, hd, generator=g).to(dt)
     want, tol = _attn_oracle(q, pool, cu, kl, table, 1 / math.sqrt(hd))
-    kw = dict(max_q=max(ql), max_kv=max(kl)) if hints else {}
+    kw = hints if isinstance(hints, dict) else dict(max_q=max(ql), max_kv=max(kl)) if hints else {}
     out = torch.full((n, hq * hd), 7.0, dtype=dt, device=dev)
     if gpu:
         q, pool = _like(q, dev), _like(pool, dev)
@@ -414,6 +414,18 @@ def test_attention_split_tiles_gpu(gpu_rt, dt, hq, hkv, hd, ql, kl):
     """More rows than the few-row body takes, over keys that are split: the splits'
     shares of such lengths are not whole 64-key tiles by themselves."""
     _check_attn(True, dt, ql, kl, hq, hkv, hd, 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,hd", [(16, 1, 128), (8, 1, 64), (12, 2, 128)])
+@pytest.mark.parametrize("ql,kl,hints", [([1], [20011], True), ([1, 1, 0], [9000, 260, 17000], True),
+                                         ([5], [12005], True), ([2, 9], [513, 7777], True),
+                                         ([30, 4], [6000, 900], dict(max_q=5, max_kv=6000)),
+                                         ([3, 1], [5000, 9000], dict(max_q=3, max_kv=4000))])
+def test_attention_joins_many_splits_gpu(gpu_rt, hq, hkv, hd, ql, kl, hints):
+    """Keys split so often that several threads join a row; requests that use few of
+    the splits; more rows and keys than the bounds that the joining is laid out for."""
+    _check_attn(True, torch.bfloat16, ql, kl, hq, hkv, hd, 16, hints=hints)
 
 
 @pytest.mark.gpu
