@@ -796,8 +796,17 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
   }
 }
 
+// Two column blocks of 128 dims take 346 registers where a CU holds one workgroup;
+// with two (256 registers) fewer LDS reads were in flight and 40 registers spilled.
+// us with two / with one: 16 requests of 4 tokens, 64 query and 8 kv heads, at up to
+// 2048 keys 35 / 30, 64 of them 97 / 82, 1 at 65535 67 / 59. (The other shapes are
+// not faster with one, and two blocks ahead in registers, 424 of them, took 32 / 88
+// / 62.)
+template <int HD, int NB>
+constexpr bool kWideFew = HD == 128 && NB == 2;
+
 template <typename T, int HD, int NB, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) k_paged_few(PagedAttnArgs a) {
+__global__ void __launch_bounds__(64 * NW, (kWideFew<HD, NB> ? 1 : 2)) k_paged_few(PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[kFewLds<HD, NB, NW> / 2];
   few_body<T, HD, NB, NW>(a, lds, blockIdx.z, blockIdx.x, blockIdx.y);
 }
@@ -948,10 +957,12 @@ hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((k_paged_mixed<T, HD, NB>), dim3((uint32_t)wgs), dim3(256), 0, s, a);
   } else {
     const dim3 grid(a.hkv, p.few_splits, a.B);
-    if (p.few_waves == 8)
-      hipLaunchKernelGGL((k_paged_few<T, HD, NB, 8>), grid, dim3(512), 0, s, a);
-    else
-      hipLaunchKernelGGL((k_paged_few<T, HD, NB, 4>), grid, dim3(256), 0, s, a);
+    if constexpr (!kWideFew<HD, NB>)
+      if (p.few_waves == 8) {
+        hipLaunchKernelGGL((k_paged_few<T, HD, NB, 8>), grid, dim3(512), 0, s, a);
+        return hipGetLastError();  // never split
+      }
+    hipLaunchKernelGGL((k_paged_few<T, HD, NB, 4>), grid, dim3(256), 0, s, a);
   }
   const uint64_t many_units = p.many_splits > 1 ? p.many_tiles : 0, few_units = p.few_splits > 1 ? a.B : 0;
   const uint64_t units = (many_units + few_units) * a.hkv;
@@ -1015,9 +1026,10 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
   p.few_splits = (uint32_t)std::min<uint64_t>((few_wgs + wgs - 1) / wgs, key_splits);
   // Short contexts of few requests: eight waves and no second launch. us with it /
   // with splits: one request of the 8B heads at 512 keys 9.4 / 11.8, at 1025 12.4 /
-  // 11.8, at 1536 15.1 / 11.6; 4 requests of 64-wide heads at 1025 8.9 / 11.6.
+  // 11.8, at 1536 15.1 / 11.6; 4 requests of 64-wide heads at 1025 8.9 / 11.6. (Two
+  // column blocks of 128 dims would spill: 21 us at 700 keys.)
   p.few_waves = 4;
-  if (only_few && p.few_splits > 1 && (uint64_t)max_kv * hd <= 96 * 1024) {
+  if (only_few && p.few_splits > 1 && (uint64_t)max_kv * hd <= 96 * 1024 && (p.few_blocks == 1 || hd == 64)) {
     p.few_waves = 8;
     p.few_splits = 1;
   }
