@@ -60,6 +60,7 @@ struct PagedAttnPlan {
   uint32_t few_splits;  // its splits of the key axis, at most
   uint32_t many_tiles;  // 128-row tiles of the other requests, at most (0: none expected)
   uint32_t many_splits;
+  uint32_t many_sorted; // 1: tiles in the order of their requests' keys (B <= 64)
   uint64_t few_part;    // rows of partial results of the few-row requests,
   uint64_t part_rows;   // and of all (hd + 2 floats each)
 };

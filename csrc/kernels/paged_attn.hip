@@ -485,14 +485,39 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
 // ---------------------------------------------------------------- many rows
 constexpr int kManyRows = 128;  // rows of a workgroup's tile: 4 waves of 32
 
-// Tile x of all tiles of the requests with more than few_rows rows, the last
-// request's last tile first (of a prompt's tiles the last sees the most keys).
-// Every wave scans the request lengths by itself, 256 a round. Returns false past
-// the end.
+// Tile x of all tiles of the requests with more than few_rows rows, a request's
+// last tile first (of a prompt's tiles the last sees the most keys), the last
+// request first. With more than one tile a CU the request with the most keys first
+// instead, so that no long tile starts late or beside another. us in request order /
+// so: 16 requests of 256 - 511 rows, 64-wide heads, at 512 - 2047 keys 66 / 57; 16 of
+// 150 - 300 (8B heads) 123 / 109; 4 of 256 - 511 at 1024 - 4096 keys 125 / 105; 12 of
+// 256 - 511 beside 36 single tokens 47 / 48 and 52 / 47, as the lengths fall. Every
+// wave scans the request lengths by itself, 256 a round. Returns false past the end.
 __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, uint32_t x, uint32_t* b, int32_t* tile) {
   constexpr int E = 4;  // requests of a lane: top - 1 - E lane - e
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t g = a.hq / a.hkv;
+  if (a.plan.many_sorted) {  // B <= 64: a lane has a request
+    const bool is = lane < a.B;
+    const int32_t end = a.cu_q[min(lane + 1, a.B)], begin = a.cu_q[min(lane, a.B)];
+    const int32_t kv = is ? a.kv_lens[lane] : 0;
+    const int32_t lo = min(max(begin, 0), (int32_t)a.n), hi = min(max(end, lo), (int32_t)a.n);
+    const uint32_t rows = is ? (uint32_t)(hi - lo) * g : 0;
+    const uint32_t tiles = rows > a.plan.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
+    uint32_t before = 0;
+    for (uint64_t left = __ballot(tiles > 0); left; left &= left - 1) {
+      const int l = __builtin_ctzll(left);
+      const int32_t other = __builtin_amdgcn_readlane(kv, l);
+      const uint32_t its = (uint32_t)__builtin_amdgcn_readlane((int)tiles, l);
+      before += other > kv || (other == kv && l < (int)lane) ? its : 0;
+    }
+    const uint64_t here = __ballot(before <= x && x - before < tiles);
+    if (!here) return false;
+    const int l = __builtin_ctzll(here);
+    *b = (uint32_t)l;
+    *tile = (int32_t)((uint32_t)__builtin_amdgcn_readlane((int)(before + tiles), l) - 1 - x);
+    return true;
+  }
   for (int32_t top = (int32_t)a.B; top > 0; top -= 64 * E) {
     const int32_t r0 = top - 1 - E * (int32_t)lane;
     int32_t cu[E + 1];  // of requests r0 + 1 - e; every index that exists is in bounds
@@ -1007,12 +1032,16 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
     // (8 heads, one kv head) at up to 8191 keys 33 / 31 / 35, 16 of 9 at 16384 43 /
     // 37 / 35, 512 rows behind 3584 (8B heads) 61 / 54 / 66; but 1040 behind 1407
     // (8 heads, one kv head) 30 / 41 / 40, 15 requests of 105 rows of 64-wide heads
-    // at 2047 32 / 35 / 35; 511 rows (8B heads) beside 32 single tokens 55 in one
+    // at 2047 32 / 35 / 35; 1024 rows of a prompt's start (8B heads) 31 in one piece,
+    // 35 in two, behind 7168 keys 182 and 148; 511 rows (8B heads) beside 32 single tokens 55 in one
     // piece, 61 in two.
     const uint64_t wgs = std::max<uint64_t>(p.many_tiles * heads, 1);
     const uint64_t one = (256 + wgs - 1) / wgs, two = (512 + wgs - 1 - std::min<uint64_t>(B * heads, 512)) / wgs;
-    const uint64_t worth = (uint64_t)max_kv * hd / (512 * 128);
+    const uint64_t keys = max_kv - std::min(max_kv, std::min(max_q, n) / 2);  // of a prompt's rows, on average
+    const uint64_t worth = keys * hd / (512 * 128);
     p.many_splits = (uint32_t)std::min(std::max(one, std::min(two, worth)), key_splits);
+    // (32 short requests in 13 splits: 31 us in request order, 33 sorted)
+    p.many_sorted = B > 1 && B <= 64 && p.many_splits <= 2 && wgs * p.many_splits > 256;
   }
   // A workgroup a CU: four waves with a block each in flight draw what HBM gives.
   // us at 128 / 256 / 512 / 1024 workgroups: 4 requests of up to 131071 keys 343 /

@@ -429,6 +429,16 @@ def test_attention_joins_many_splits_gpu(gpu_rt, hq, hkv, hd, ql, kl, hints):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,hd", [(32, 32, 64), (64, 16, 128)])
+@pytest.mark.parametrize("hints", [False, True])
+def test_attention_sorted_tiles_gpu(gpu_rt, hq, hkv, hd, hints):
+    """More tiles than CUs: they are taken in the order of their requests' keys, equal
+    ones among them, beside requests without tiles."""
+    _check_attn(True, torch.bfloat16, [130, 1, 0, 200, 64, 200, 33], [300, 90, 5, 450, 64, 450, 1000], hq, hkv, hd, 16,
+                hints=hints, extra_rows=5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("sharp", [0.0, 30.0])
 def test_attention_flat_and_peaked_gpu(gpu_rt, sharp):
     """All scores equal; scores whose maximum moves far from tile to tile."""
