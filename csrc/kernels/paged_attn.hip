@@ -1051,7 +1051,9 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
   // tiles fill the CUs too (12 x 511 rows and 36 single tokens of 64-wide heads at
   // up to 2047 keys: 53 us with two splits and their joining, 49.6 without; a token
   // each of 4 requests at 131071 and a chunk: 113, and 142 at 64 workgroups).
-  const uint64_t wgs = std::max<uint64_t>(B * heads, 1), few_wgs = only_few ? 256 : 128;
+  // Not at all for one request, which the bound says has more rows (4096 rows of a
+  // prompt behind 4095 keys: 5 us of joining nothing).
+  const uint64_t wgs = std::max<uint64_t>(B * heads, 1), few_wgs = only_few ? 256 : B > 1 ? 128 : 1;
   p.few_splits = (uint32_t)std::min<uint64_t>((few_wgs + wgs - 1) / wgs, key_splits);
   // Short contexts of few requests: eight waves and no second launch. us with it /
   // with splits: one request of the 8B heads at 512 keys 9.4 / 11.8, at 1025 12.4 /
