@@ -1026,20 +1026,32 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
   } else {
     // 0 rows where one token already takes more
     p.few_rows = g <= 32 ? 16 * p.few_blocks : 0;
-    p.many_tiles = (uint32_t)(n * g / kManyRows + std::min<uint64_t>(B, n * g / (p.few_rows + 1)));
-    // One workgroup a CU; two, those of single tokens among them, where each keeps
-    // 512 keys of 128 dims (fewer do not pay for its start). us at 256 / 512 / 768 workgroups: 32 requests of 5 rows
-    // (8 heads, one kv head) at up to 8191 keys 33 / 31 / 35, 16 of 9 at 16384 43 /
-    // 37 / 35, 512 rows behind 3584 (8B heads) 61 / 54 / 66; but 1040 behind 1407
-    // (8 heads, one kv head) 30 / 41 / 40, 15 requests of 105 rows of 64-wide heads
-    // at 2047 32 / 35 / 35; 1024 rows of a prompt's start (8B heads) 31 in one piece,
-    // 35 in two, behind 7168 keys 182 and 148; 511 rows (8B heads) beside 32 single tokens 55 in one
-    // piece, 61 in two.
+    // m requests of r_i rows have at most floor((sum r_i + 127 m) / 128) tiles
+    const uint64_t at_most = std::min<uint64_t>(B, n * g / (p.few_rows + 1));
+    p.many_tiles = (uint32_t)((n * g + (kManyRows - 1) * at_most) / kManyRows);
+    // The number of splits with the least expected time, in us: a workgroup's share of
+    // the keys (a prompt's rows see about three quarters of its own) at what a tile of
+    // them takes alone on its CU, longer by half beside a second workgroup; the join;
+    // partial results written and read at 7 TB/s (they stay in the caches). us measured
+    // with 1 / 2 / 3 / 4 / 6 / 8 / 12 splits, the chosen one in brackets:
+    //   512 rows of a prompt's start, 8B heads      [18] 24 26 26 28 32 36
+    //   2 x 42 rows behind 1508, 24:8 heads          38 27 22 20 18 [18] 18
+    //   25 x 58 - 116 rows of 8:1 at up to 545      [23] 28 26 36 31 53 46
+    //   2 x 220 rows behind 2198, 16:4, 64 wide      36 25 22 20 [20] 21 22
+    //   1024 rows behind 7168, 8B heads             182 [148] 157 156
+    // and 32 x 5 rows of 8:1 at up to 8191 37 / 33 / 31 with 6 / 8 / 12.
     const uint64_t wgs = std::max<uint64_t>(p.many_tiles * heads, 1);
-    const uint64_t one = (256 + wgs - 1) / wgs, two = (512 + wgs - 1 - std::min<uint64_t>(B * heads, 512)) / wgs;
-    const uint64_t keys = max_kv - std::min(max_kv, std::min(max_q, n) / 2);  // of a prompt's rows, on average
-    const uint64_t worth = keys * hd / (512 * 128);
-    p.many_splits = (uint32_t)std::min(std::max(one, std::min(two, worth)), key_splits);
+    const double keys = std::max<double>(max_kv - std::min(max_q, n) / 4.0, 1.0);
+    double best = 0.0;
+    for (uint32_t splits = 1; splits <= std::min<uint64_t>(key_splits, 64); ++splits) {
+      const double load = (double)wgs * splits / 256.0;  // workgroups a CU
+      double us = keys * (hd == 64 ? 0.010 : 0.0165) / splits * (load <= 1 ? 1.0 : load <= 2 ? 0.5 + 0.5 * load : 0.75 * load);
+      if (splits > 1) us += 3.0 + (double)n * hq * splits * (hd + 2) * 8 / 7e6;
+      if (splits == 1 || us < best) {
+        best = us;
+        p.many_splits = splits;
+      }
+    }
     // (32 short requests in 13 splits: 31 us in request order, 33 sorted)
     p.many_sorted = B > 1 && B <= 64 && p.many_splits <= 2 && wgs * p.many_splits > 256;
   }
