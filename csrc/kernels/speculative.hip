@@ -92,8 +92,8 @@ __device__ __forceinline__ void weights(const VerifyRow<T>& r, uint32_t i0, uint
   const bool no_q = whole || !r.q;
   T p[N], q[N];
   constexpr uint32_t E = 16 / sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(E)));
-  if (step == 1 && i0 + N <= V && (((uintptr_t)(r.p + i0) | (uintptr_t)(qr + i0)) & 15) == 0) {
+  typedef T vec __attribute__((ext_vector_type(E), aligned(sizeof(T))));  // rows of an odd length begin anywhere
+  if (step == 1 && i0 + N <= V) {
     // consecutive entries: 16 bytes a load, or the lanes' 64-byte stride costs a
     // cache line for each of them
 #pragma unroll
@@ -115,14 +115,14 @@ __device__ __forceinline__ void weights(const VerifyRow<T>& r, uint32_t i0, uint
 }
 
 // Sum of the calling wave's quarter of a chunk: 16 entries a lane, all loads in
-// flight before the first use, 16 bytes each where both rows allow.
+// flight before the first use, 16 bytes each but in the row's last quarter.
 template <typename T>
 __device__ __forceinline__ double quarter_sum(const VerifyRow<T>& r, uint32_t i0, uint32_t V) {
   constexpr uint32_t E = 16 / sizeof(T), N = kVerifyChunk / 4 / 64 / E;  // entries of a load, loads
-  typedef T vec __attribute__((ext_vector_type(E)));
+  typedef T vec __attribute__((ext_vector_type(E), aligned(sizeof(T))));
   const uint32_t lane = threadIdx.x & 63;
   double sum = 0.0;
-  if (i0 + kVerifyChunk / 4 <= V && ((((uintptr_t)(r.p + i0)) | (r.q ? (uintptr_t)(r.q + i0) : 0)) & 15) == 0) {
+  if (i0 + kVerifyChunk / 4 <= V) {
     vec p[N], q[N];
 #pragma unroll
     for (uint32_t k = 0; k < N; ++k) p[k] = *reinterpret_cast<const vec*>(r.p + i0 + (k * 64 + lane) * E);
