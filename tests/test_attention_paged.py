@@ -811,6 +811,48 @@ def test_captured_step_gpu(gpu_rt):
 
 
 @pytest.mark.gpu
+def test_captured_padded_batch_gpu(gpu_rt):
+    """One captured call over a padded batch, replayed over other divisions of its rows:
+    single tokens, drafts, a chunk, rows of nobody (left as they were)."""
+    g = torch.Generator().manual_seed(21)
+    n, hq, hkv, hd, P, dt = 200, 16, 2, 128, 16, torch.bfloat16
+    q = torch.randn(n, hq, hd, generator=g).to(dt)
+    batches = [([1, 1, 1, 1], [900, 3, 2000, 64]), ([100, 1, 0, 90], [1500, 17, 40, 90]), ([5, 3, 190, 2], [700, 3, 2047, 2]),
+               ([0, 0, 0, 0], [5, 0, 9, 1]), ([1, 0, 1, 0], [1, 0, 2048, 7])]
+    table, _, num = _requests([1] * 4, [2048] * 4, P)
+    pool = torch.randn(2, num, hkv, P, hd, generator=g).to(dt)
+    qd, pd, td = q.cuda(), pool.cuda(), table.cuda()
+    cu, kv = _i32([0] * 5, "cuda"), _i32([0] * 4, "cuda")
+    out = torch.zeros(n, hq * hd, dtype=dt, device="cuda")
+
+    def call():
+        return paged.attention(qd, pd, cu, kv, td, out=out)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for ql, kl in batches + batches[::-1]:
+        c = [sum(ql[:i]) for i in range(5)]
+        cu.copy_(_i32(c, "cuda"))
+        kv.copy_(_i32(kl, "cuda"))
+        out.fill_(7.0)
+        graph.replay()
+        got = out.cpu().double()
+        assert (got[c[-1]:] == 7.0).all()
+        if c[-1]:
+            want, tol = _attn_oracle(q[:c[-1]], pool, c, kl, table, 1 / math.sqrt(hd))
+            assert ((got[:c[-1]] - want).abs() <= tol).all(), (ql, kl)
+        out.fill_(9.0)
+        call()
+        assert torch.equal(out.cpu().double()[:c[-1]], got[:c[-1]])
+
+
+@pytest.mark.gpu
 def test_two_streams_gpu(gpu_rt):
     """Calls on two streams at once do not share a workspace."""
     g = torch.Generator().manual_seed(8)
