@@ -26,6 +26,18 @@
 // four waves of 32 rows share each tile of 64 keys (128 of 64 dims). One launch
 // serves both kinds in a mixed batch. The key axis is split where rows are few;
 // k_paged_combine joins the parts.
+//
+// Probabilities enter the second product in the element type; the row's sum takes
+// them in f32. `few` multiplies with what that rounding left over as well (a second
+// operand, 2 x 16 bits): its matrix cores wait for memory, and a single token gets
+// what the contiguous cache's kernel gives, whose probabilities stay in f32. Error
+// against f64 (norm of the difference over the norm) without / with it, and us: 64
+// tokens of 64:8 heads at up to 2048 keys, bf16, 2.14e-3 / 1.66e-3 (1.66e-3 is the
+// output's own rounding), 67.1 / 67.2; 4 x 1 at 131071, fp16, 2.84e-4 / 2.09e-4, 260
+// / 260; 64 x 4 70B rows 80 / 82.5; 4 x 1 at 300, 64-wide, 6.5 / 6.6. `many` is
+// bound by the matrix cores and keeps the type's bits: with the second operand 4096
+// rows behind 4095 keys take 560 us for 415 (1.66e-3 for 2.35e-3), 12 x 511 + 36 x 1
+// 64-wide 59 for 49 (2.07e-4 for 2.89e-4), 32 x 5 rows 35.7 for 31.3.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -79,6 +91,13 @@ template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   typename Vec<T>::v2 v = {from_f32<T>(a), from_f32<T>(b)};
   return __builtin_bit_cast(uint32_t, v);
+}
+// What pack2 rounded away, as a second pair: the two add up to a and b but for the
+// square of the type's half step (2^-16 of bf16, 2^-22 of fp16).
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_rest(float a, float b, uint32_t packed) {
+  const typename Vec<T>::v2 v = __builtin_bit_cast(typename Vec<T>::v2, packed);
+  return pack2<T>(a - to_f32<T>(v[0]), b - to_f32<T>(v[1]));
 }
 
 // Any infinity or NaN among 8 elements?
@@ -334,7 +353,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
           for (int nb = 0; nb < NB; ++nb) s[t][nb] = Mma<T>::m16(ka, qf[nb][k], s[t][nb]);
         }
       }
-      u32x4 p[NB];
+      u32x4 p[NB], rest[NB];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         float x[8];
@@ -373,7 +392,10 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
           l[nb] += x[j];
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[nb][j] = pack2<T>(x[2 * j], x[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) {
+          p[nb][j] = pack2<T>(x[2 * j], x[2 * j + 1]);
+          rest[nb][j] = pack2_rest<T>(x[2 * j], x[2 * j + 1], p[nb][j]);
+        }
       }
       // O^T += V^T P^T, keys in the order of P's registers: 4 quad .. + 3 of each 16-key tile
       auto v_frag = [&](int d) {
@@ -385,6 +407,8 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
         const u32x4 va = v_frag(d);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) o[nb][d] = Mma<T>::m16(va, p[nb], o[nb][d]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) o[nb][d] = Mma<T>::m16(va, rest[nb], o[nb][d]);
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();

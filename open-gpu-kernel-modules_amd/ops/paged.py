@@ -197,6 +197,13 @@ def attention(q: torch.Tensor, pages: torch.Tensor, cu_q: torch.Tensor, kv_lens:
     last page, a later token) cannot reach a result, NaN or not. Rows that would
     need a page outside the pool or beyond their table row give NaN.
 
+    Scores, maxima, sums and the result before its one rounding are f32. A single
+    token's probabilities (of up to 32 query heads a kv head), and a draft's where no
+    request of the batch may have more than 32 rows per kv head (``max_q``), are
+    multiplied with twice the type's bits, so that such a call is as exact as
+    ``fused.attention``. Those of longer chunks are rounded to the type, which adds an
+    error of up to half a step of it relative to sum p |v|.
+
     ``max_q`` / ``max_kv``: the host's bounds of rows and length per request; they
     only choose how the work is split (default: n and the table's width). ``out``
     shares no memory with q or the pool. Limits: 65535 requests, 2^30 tokens each."""
