@@ -3,10 +3,13 @@
 from __future__ import annotations
 
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
 
+from ogkm.ops import decode as D
 from ogkm.ops import paged
 from test_attention_paged import _attn_oracle, _dev, _i32, _requests
 
@@ -62,3 +65,127 @@ def test_probability_bits_gpu(gpu_rt, dt, hq, hkv, hd, ql, kl):
 @pytest.mark.parametrize("ql,kl,chunk", [([3, 4], [601, 88], 0), ([70, 1, 1], [70, 800, 2000], 70)])
 def test_probability_bits_of_drafts_and_beside_a_chunk_gpu(gpu_rt, dt, ql, kl, chunk):
     _check_probability_bits(True, dt, ql, kl, 8, 1, 128, 16, chunk)
+
+
+# ---------------------------------------------------------------- the documented step
+def _documented_step():
+    """The server's step as README.md gives it."""
+    text = (Path(__file__).resolve().parents[1] / "README.md").read_text()
+    return next(c for c in re.findall(r"```python\n(.*?)```", text, re.S) if "verify_draft" in c)
+
+
+class _Layer:
+    def __init__(self, pages):
+        self.pages = pages
+
+    def qkv(self, x):
+        return x
+
+    def rest(self, x, out):
+        self.out = out
+        return x
+
+
+# Of each request: new tokens, drafts among them, how many of those the target keeps. Request 2
+# wants more pages than there are until the last step, and its rows are cached all the while.
+STEPS = [([4, 40, 3], [3, 0, 2], [1, 0, 2]), ([1, 3, 400], [0, 2, 0], [0, 0, 0]), ([5, 1, 400], [4, 0, 0], [4, 0, 0]),
+         ([2, 5, 30], [1, 4, 0], [0, 2, 0])]
+GRANTED = [[1, 1, 1], [1, 1, 0], [1, 1, 0], [1, 1, 1]]
+
+
+class _Loop:
+    """State that the documented step runs on, static, so that a captured step finds it again."""
+
+    def __init__(self, dev, n):
+        B, K, V, hq, hkv, hd, P = 3, 4, 50, 4, 2, 64, 16
+        z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
+        self.B, self.K, self.V, self.P, self.hkv = B, K, V, P, hkv
+        layer = _Layer(torch.full((2, 16, hkv, P, hd), math.nan, dtype=torch.bfloat16, device=dev))
+        cos, sin = D.rope_tables(hd, 1024, 500000.0, dev)
+        self.s = dict(new_lens=z(B), kv_lens=z(B), page_counts=z(B), block_table=z(B, 32) - 1,
+                      free_pages=torch.arange(15, -1, -1, dtype=torch.int32).to(dev), free_start=z(1), counts=z(B),
+                      x=torch.zeros(n, (hq + 2 * hkv) * hd, dtype=torch.bfloat16, device=dev), drafts=z(B, K),
+                      probs=torch.zeros(B, K + 1, V, device=dev), u=torch.full((B, K), 0.5, device=dev),
+                      u_last=torch.zeros(B, device=dev))
+        self.fixed = dict(layers=[layer], cos=cos, sin=sin, page_size=P, n_tokens=n, hq=hq, hkv=hkv, max_q=n,
+                          max_kv=512, draft_probs=None)
+        self.code = compile(_documented_step(), "README.md", "exec")
+
+    def call(self):
+        env = {**self.s, **self.fixed}
+        exec(self.code, env)
+        for name in ("kv_lens", "page_counts", "free_start"):
+            self.s[name].copy_(env[name])
+        return env["plan"].granted, env["accepted"]
+
+    def feed(self, step, g):
+        """Inputs of a step: random rows; probabilities that keep the said number of drafts."""
+        new, drafts, kept = step
+        x = torch.randn(self.s["x"].shape, generator=g).bfloat16()
+        self.s["x"].copy_(x)
+        self.s["new_lens"].copy_(torch.tensor(new, dtype=torch.int32))
+        self.s["counts"].copy_(torch.tensor(drafts, dtype=torch.int32))
+        self.s["drafts"].copy_(torch.arange(self.B * self.K, dtype=torch.int32).view(self.B, self.K))
+        p = torch.zeros(self.B, self.K + 1, self.V)
+        p[:, :, -1] = 1
+        for b in range(self.B):
+            for j in range(kept[b]):
+                p[b, j] = 0
+                p[b, j, b * self.K + j] = 1
+        self.s["probs"].copy_(p)
+        return x
+
+    def check(self, lens, rows):
+        """Lengths, and v of every cached token, which is stored as it came."""
+        assert self.s["kv_lens"].tolist() == lens
+        pool, table = self.fixed["layers"][0].pages.cpu(), self.s["block_table"].tolist()
+        for b, r in enumerate(rows):
+            for t, v in enumerate(r):
+                assert torch.equal(pool[1, table[b][t // self.P], :, t % self.P].flatten(), v), (b, t)
+
+
+def _run_documented_steps(loop, call, g):
+    lens, rows, width = [0] * 3, [[] for _ in range(3)], loop.s["x"].shape[1]
+    for step, granted in zip(STEPS, GRANTED):
+        x = loop.feed(step, g)
+        got, accepted = call()
+        assert got.tolist() == granted
+        at = 0
+        for b, (new, drafts, kept) in enumerate(zip(*step)):
+            if granted[b]:
+                take = new - drafts + kept
+                rows[b] += list(x[at:at + take, width - loop.hkv * 64:])
+                lens[b] += take
+                assert accepted.tolist()[b] == kept
+            at += new
+        loop.check(lens, rows)
+
+
+def test_documented_step_cpu(fake_rt):
+    """Drafts, prompt chunks and requests without pages in one batch: a refused
+    request keeps its length and its rows, a chunk keeps all of its own."""
+    _run_documented_steps(loop := _Loop("cpu", 410), loop.call, torch.Generator().manual_seed(2))
+
+
+@pytest.mark.gpu
+def test_documented_step_captured_gpu(gpu_rt):
+    """The same as one captured step, replayed."""
+    loop = _Loop("cuda", 410)
+    start = {k: v.clone() for k, v in loop.s.items()}
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        loop.call()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = loop.call()
+    for turn in range(3):
+        for k, v in start.items():
+            loop.s[k].copy_(v)
+
+        def call():
+            graph.replay()
+            return outs
+
+        _run_documented_steps(loop, call, torch.Generator().manual_seed(turn))
