@@ -17,6 +17,9 @@ namespace ogkm {
 //   need_b  = max(0, ceil((kv_b + new_b) / P) - held_b)
 //   upto_b  = sum of need up to b                  (free-list entries of b: [upto_b - need_b, upto_b))
 //   granted = the pages fit the table row and the free list, the rows fit n_tokens
+//             (a refused request's pages stay in upto: those behind it that lack
+//             pages are refused too and cannot overtake it; prefix sums do not
+//             depend on what was granted, a first-fit rule would be sequential)
 // The op moves a few KB: its time is one launch and a chain of four dependent
 // memory rounds (lengths -> scan -> table or free list -> store). So it is ONE
 // launch: every workgroup scans all requests by itself (LDS keeps 9 bytes of

@@ -90,9 +90,17 @@ def _unaligned(op: str):
 
 class Plan(NamedTuple):
     """One step of a batch, all int32 on the device. ``granted[b]`` is 0 where
-    request b's pages did not fit the free list or its table row, or its rows
-    did not fit n_tokens: its lengths and pages then stay as they were and its
-    rows have position and slot -1."""
+    request b's tokens do not fit its table row, where its rows end behind
+    n_tokens, or where it lacks pages and those asked for up to it, its own among
+    them, are more than the free list has: its lengths and pages then stay as they
+    were and its rows have position and slot -1.
+
+    Pages are asked for in request order, and a request that finds too few keeps its
+    place: those behind it that lack pages are refused too, however few they lack,
+    so that small requests never overtake a large one for good. (One that does not
+    fit its table row or the batch asks for none.) A server therefore puts running
+    requests before those it admits, and takes a refused admission out of the next
+    batches (0 new tokens) until pages came back."""
 
     cu_q: torch.Tensor         # [B + 1] first row of each request
     kv_lens: torch.Tensor      # [B] cached tokens after the step

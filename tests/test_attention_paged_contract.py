@@ -189,3 +189,32 @@ def test_documented_step_captured_gpu(gpu_rt):
             return outs
 
         _run_documented_steps(loop, call, torch.Generator().manual_seed(turn))
+
+
+# ---------------------------------------------------------------- who gets pages
+def _granted(gpu, new, kv, held, free, width=40):
+    dev, B = _dev(gpu), len(new)
+    p = paged.plan(_i32(new, dev), _i32(kv, dev), _i32(held, dev), torch.zeros(B, width, dtype=torch.int32, device=dev),
+                   torch.arange(100, 100 + free, dtype=torch.int32).to(dev), _i32([0], dev), 16, sum(new))
+    return p.granted.tolist(), p.page_counts.tolist(), p.free_start.tolist()
+
+
+def _check_refusals(gpu):
+    # 25 pages of 10: the single pages behind it are not handed out either
+    assert _granted(gpu, [400, 1, 1], [0, 16, 0], [0, 1, 0], 10) == ([0, 0, 0], [0, 1, 0], [0])
+    # a request that lacks none is not concerned
+    assert _granted(gpu, [400, 1, 1], [0, 7, 0], [0, 1, 0], 10) == ([0, 1, 0], [0, 1, 0], [0])
+    # behind the running ones, or left out, it stops nobody
+    assert _granted(gpu, [1, 1, 400], [16, 0, 0], [1, 0, 0], 10) == ([1, 1, 0], [2, 1, 0], [2])
+    assert _granted(gpu, [0, 1, 1], [0, 16, 0], [0, 1, 0], 10) == ([1, 1, 1], [0, 2, 1], [2])
+    # nor does one that its table row has no room for
+    assert _granted(gpu, [400, 1, 1], [0, 16, 0], [0, 1, 0], 10, width=4) == ([0, 1, 1], [0, 2, 1], [2])
+
+
+def test_a_refused_request_keeps_its_place_cpu(fake_rt):
+    _check_refusals(False)
+
+
+@pytest.mark.gpu
+def test_a_refused_request_keeps_its_place_gpu(gpu_rt):
+    _check_refusals(True)
