@@ -200,8 +200,9 @@ def attention(q: torch.Tensor, pages: torch.Tensor, cu_q: torch.Tensor, kv_lens:
               scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """q [n, hq, hd] (rotated), rows [cu_q[b], cu_q[b + 1]) of request b being its last
     new tokens of the ``kv_lens[b]`` cached ones -> [n, hq * hd]: row i of a request
-    sees its tokens 0 .. kv_lens - rows + i. A row that sees nothing gives 0; rows
-    behind cu_q[B] are left as they are in ``out``. What no row sees (the rest of a
+    sees its tokens 0 .. kv_lens - rows + i. A row that sees nothing gives 0. ``cu_q``
+    ascends; bounds outside q are cut to it, and rows of no request (those behind
+    cu_q[B]) are left as they are in ``out``. What no row sees (the rest of a
     last page, a later token) cannot reach a result, NaN or not. Rows that would
     need a page outside the pool or beyond their table row give NaN.
 

@@ -218,3 +218,45 @@ def test_a_refused_request_keeps_its_place_cpu(fake_rt):
 @pytest.mark.gpu
 def test_a_refused_request_keeps_its_place_gpu(gpu_rt):
     _check_refusals(True)
+
+
+# ---------------------------------------------------------------- row bounds
+def _check_row_bounds(gpu, n, raw, cut, kl, hq, hkv, hd):
+    """Row bounds outside q are cut to it: the same results as with `cut`, and rows that
+    belong to no request stay as they were."""
+    dev, dt, g = _dev(gpu), torch.bfloat16, torch.Generator().manual_seed(n)
+    table, _, num = _requests([1] * len(kl), kl, 16)
+    q = torch.randn(n, hq, hd, generator=g).to(dt)
+    pool = torch.randn(2, num, hkv, 16, hd, generator=g).to(dt)
+    want, tol = torch.full((n, hq * hd), 7.0, dtype=torch.float64), torch.zeros(n, hq * hd, dtype=torch.float64)
+    for b, (lo, hi) in enumerate(cut):
+        if lo == hi:
+            continue
+        w, t = _attn_oracle(q[lo:hi], pool, [0, hi - lo], [kl[b]], table[b:b + 1], 1 / math.sqrt(hd))
+        want[lo:hi], tol[lo:hi] = w, t
+    for hints in ({}, dict(max_q=n, max_kv=max(kl)), dict(max_q=1, max_kv=1)):
+        out = torch.full((n, hq * hd), 7.0, dtype=dt, device=dev)
+        got = paged.attention(q.to(dev), pool.to(dev), _i32(raw, dev), _i32(kl, dev), table.to(dev), out=out, **hints)
+        assert ((got.cpu().double() - want).abs() <= tol).all(), hints
+
+
+# rows of q, bounds as given, rows of each request after the cut, lengths
+BOUNDS = [
+    (7, [-4, 1, 4, 5, 100], [(0, 1), (1, 4), (4, 5), (5, 7)], [40, 50, 10, 33]),
+    (7, [5, 2, 7], [(5, 5), (2, 7)], [40, 50]),  # falling: the first request has no rows, rows 0 and 1 nobody
+    (7, [2, 3, 3, 4], [(2, 3), (3, 3), (3, 4)], [9, 50, 64]),
+    (90, [-2**31, 1, 80, 2**31 - 1], [(0, 1), (1, 80), (80, 90)], [300, 100, 700]),
+    (90, [60, 50, 90], [(60, 60), (50, 90)], [40, 90]),
+]
+
+
+@pytest.mark.parametrize("n,raw,cut,kl", BOUNDS)
+def test_row_bounds_cpu(fake_rt, n, raw, cut, kl):
+    _check_row_bounds(False, n, raw, cut, kl, 4, 2, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,hd", [(4, 2, 64), (16, 1, 128), (40, 1, 64)])
+@pytest.mark.parametrize("n,raw,cut,kl", BOUNDS)
+def test_row_bounds_gpu(gpu_rt, n, raw, cut, kl, hq, hkv, hd):
+    _check_row_bounds(True, n, raw, cut, kl, hq, hkv, hd)
