@@ -59,7 +59,7 @@ struct Mma;
 template <>
 struct Mma<__bf16> {
   typedef Vec<__bf16>::v8 v8;
-  static constexpr uint32_t kExp = 0x7F807F80u, kOne = 0x00800080u;  // exponent bits of a pair, their lowest
+  static constexpr uint32_t kInf = 0x7F80u;  // exponent bits
   static __device__ __forceinline__ f32x4_t m16(u32x4 a, u32x4 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
@@ -70,7 +70,7 @@ struct Mma<__bf16> {
 template <>
 struct Mma<_Float16> {
   typedef Vec<_Float16>::v8 v8;
-  static constexpr uint32_t kExp = 0x7C007C00u, kOne = 0x04000400u;
+  static constexpr uint32_t kInf = 0x7C00u;
   static __device__ __forceinline__ f32x4_t m16(u32x4 a, u32x4 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
@@ -100,17 +100,30 @@ __device__ __forceinline__ uint32_t pack2_rest(float a, float b, uint32_t packed
   return pack2<T>(a - to_f32<T>(v[0]), b - to_f32<T>(v[1]));
 }
 
-// Any infinity or NaN among 8 elements?
-template <typename T>
-__device__ __forceinline__ bool nonfinite(u32x4 x) {
-  uint32_t hit = 0;
+// Any infinity or NaN among N x 8 elements? Two by an instruction: a small multiple of
+// each, added up in f32, stays finite exactly if all are (64 of 2^128 2^-100, or 65504).
+__device__ __forceinline__ float add_dot(Vec<__bf16>::v2 a, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(a, __builtin_bit_cast(Vec<__bf16>::v2, 0x0D800D80u), c, false);  // 2^-100
+}
+__device__ __forceinline__ float add_dot(Vec<_Float16>::v2 a, float c) {
+  return __builtin_amdgcn_fdot2(a, __builtin_bit_cast(Vec<_Float16>::v2, 0x3C003C00u), c, false);  // 1
+}
+template <typename T, int N>
+__device__ __forceinline__ bool any_nonfinite(const u32x4 (&x)[N]) {
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) hit |= (x[j] & Mma<T>::kExp) + Mma<T>::kOne;
-  return (hit & 0x80008000u) != 0;
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t pair = x[i][j];  // a bit_cast of x[i][j] itself would read x[i][0]
+      s[j] = add_dot(__builtin_bit_cast(typename Vec<T>::v2, pair), s[j]);
+    }
+  return !(fabsf((s[0] + s[1]) + (s[2] + s[3])) < __builtin_inff());
 }
 
-// V with infinities or NaNs in a tile that some row does not see whole: there a
-// probability of 0 times such a value would be NaN. Such a value is taken out
+// V with infinities or NaNs in a tile that some row does not see whole (a probability
+// of 0 times such a value would be NaN), and in every block of the few-row body (an
+// infinity times what a probability's rounding left, 0 or of either sign). Such a value is taken out
 // of V, and the first key that has one is kept for each dim and kind (NaN, +inf,
 // -inf) in LDS: a row sees keys 0 .. pos, so it sees one exactly if pos is not
 // before that key, and special() adds what it does to the row's sum.
@@ -118,7 +131,7 @@ constexpr int32_t kNever = INT32_MAX;
 template <typename T, int HD>
 __device__ __forceinline__ void take_special(u32x4* v8, int32_t key, uint32_t dim, int32_t* first_key) {
   u32x4 x = *v8;
-  constexpr uint32_t inf = Mma<T>::kExp & 0xFFFFu;
+  constexpr uint32_t inf = Mma<T>::kInf;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -316,11 +329,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, uint16_t* lds, 
       const bool miss0 = missing[0], miss1 = missing[1];
       const int32_t t0 = c0 + (n * NW + (int32_t)wave) * 32;
       const bool masked = t0 + 31 > first;
-      bool odd = false;
-      if (masked) {
-#pragma unroll
-        for (int j = 0; j < 2 * LD; ++j) odd |= nonfinite<T>(vr[j]);
-      }
+      const bool odd = any_nonfinite<T>(vr);
 #pragma unroll
       for (int j = 0; j < 2 * LD; ++j) {  // 512 / HD rows by each wave-wide store
         *reinterpret_cast<u32x4*>(kw + j * (512 / HD) * kKRow<HD>) = kr[j];
@@ -699,11 +708,7 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
     const int32_t t0 = c0 + i * KT;
     uint16_t* buf = lds + (i & 1) * kTile;
     const bool tile_masked = t0 + KT - 1 > first;
-    bool odd = false;
-    if (tile_masked) {
-#pragma unroll
-      for (int j = 0; j < LJ; ++j) odd |= nonfinite<T>(vr[j]);
-    }
+    const bool odd = tile_masked && any_nonfinite<T>(vr);
 #pragma unroll
     for (int j = 0; j < LJ; ++j) {
       *reinterpret_cast<u32x4*>(buf + kw + j * (2048 / HD) * kKRow<HD>) = kr[j];

@@ -260,3 +260,44 @@ def test_row_bounds_cpu(fake_rt, n, raw, cut, kl):
 @pytest.mark.parametrize("n,raw,cut,kl", BOUNDS)
 def test_row_bounds_gpu(gpu_rt, n, raw, cut, kl, hq, hkv, hd):
     _check_row_bounds(True, n, raw, cut, kl, hq, hkv, hd)
+
+
+# ---------------------------------------------------------------- infinities that every row sees
+def _check_seen_infinities(gpu, dt, m, kv, hq, hkv, hd):
+    """V with infinities or NaN in early tokens: each row's result is that value in its
+    dim (NaN where both signs meet), and the other dims are right. Scores stay within
+    a few units, so no weight is lost in f32."""
+    dev, g = _dev(gpu), torch.Generator().manual_seed(m + kv)
+    table, cu, num = _requests([m], [kv], 16)
+    q = torch.randn(m, hq, hd, generator=g).to(dt)
+    pool = torch.randn(2, num, hkv, 16, hd, generator=g).to(dt)
+    want, tol = _attn_oracle(q, pool, cu, [kv], table, 1 / math.sqrt(hd))
+    want = want.view(m, hq, hd)
+    inf = math.inf
+    for t, d, v, total in ((5, 3, inf, inf), (1, hd - 1, -inf, -inf), (0, 7, inf, math.nan), (6, 7, -inf, math.nan),
+                           (2, 9, math.nan, math.nan), (3, 11, inf, inf), (4, 11, inf, inf)):
+        pool[1, table[0, 0], :, t, d] = v
+        want[:, :, d] = total
+    want = want.view(m, hq * hd)
+    got = paged.attention(q.to(dev), pool.to(dev), _i32(cu, dev), _i32([kv], dev), table.to(dev)).cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    fine = torch.isfinite(want)
+    assert ((got - want).abs()[fine] <= tol[fine]).all()
+
+
+SEEN = [(1, 7), (1, 300), (3, 70), (4, 1500), (40, 200), (150, 900)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,kv", SEEN[:4])
+def test_seen_infinities_cpu(fake_rt, dt, m, kv):
+    _check_seen_infinities(False, dt, m, kv, 4, 2, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,hd", [(4, 4, 64), (8, 1, 128), (24, 1, 64)])
+@pytest.mark.parametrize("m,kv", SEEN)
+def test_seen_infinities_gpu(gpu_rt, dt, m, kv, hq, hkv, hd):
+    _check_seen_infinities(True, dt, m, kv, hq, hkv, hd)
