@@ -21,8 +21,8 @@
 // Two bodies. `few` (up to 32 rows per kv head: single tokens, drafts) is bound
 // by the KV bytes: each wave streams its own 32-key blocks through wave-private
 // LDS without barriers, the waves join at the end. 64 tokens of 64 query and 8 kv
-// heads at up to 2048 keys: 69 us; 4 tokens of 32 / 8 heads at up to 131071: 258
-// us, 5.6 TB/s of K and V. `many` (prompt chunks) is bound by the matrix cores:
+// heads at up to 2048 keys: 68 - 71 us; 4 tokens of 32 / 8 heads at up to 131071:
+// 260 us, 5.6 TB/s of K and V. `many` (prompt chunks) is bound by the matrix cores:
 // four waves of 32 rows share each tile of 64 keys (128 of 64 dims). One launch
 // serves both kinds in a mixed batch. The key axis is split where rows are few;
 // k_paged_combine joins the parts.
@@ -33,8 +33,9 @@
 // what the contiguous cache's kernel gives, whose probabilities stay in f32. Error
 // against f64 (norm of the difference over the norm) without / with it, and us: 64
 // tokens of 64:8 heads at up to 2048 keys, bf16, 2.14e-3 / 1.66e-3 (1.66e-3 is the
-// output's own rounding), 67.1 / 67.2; 4 x 1 at 131071, fp16, 2.84e-4 / 2.09e-4, 260
-// / 260; 64 x 4 70B rows 80 / 82.5; 4 x 1 at 300, 64-wide, 6.5 / 6.6. `many` is
+// output's own rounding), 67.0 / 67.9; 4 x 1 at 131071, fp16, 2.84e-4 / 2.09e-4, 259
+// / 260; 64 x 4 70B rows 77.7 / 81.3; 1 x 1 at 1025 keys 9.7 / 9.9; 4 x 1 at 1025,
+// 64-wide, 9.0 / 9.7; single tokens beside chunks, up to 6 % of the call. `many` is
 // bound by the matrix cores and keeps the type's bits: with the second operand 4096
 // rows behind 4095 keys take 560 us for 415 (1.66e-3 for 2.35e-3), 12 x 511 + 36 x 1
 // 64-wide 59 for 49 (2.07e-4 for 2.89e-4), 32 x 5 rows 35.7 for 31.3.
@@ -597,8 +598,8 @@ constexpr float kLazy = 6.f;
 // A wave owns 32 rows, the workgroup walks tiles of 8192 / HD keys in two LDS
 // buffers: tile i + 1 flies into registers while tile i is multiplied, one barrier a tile
 // (a buffer is written two tiles after it was read). 4096 rows behind 4095 cached
-// keys of the 8B heads: 413 us, 1000 TFLOP/s, where the library's 8192^3 product
-// of such values reaches 1140 - 1230 on this card. The wave alternates between
+// keys of the 8B heads: 414 - 451 us on different cards, 995 - 914 TFLOP/s, where the
+// library's 8192^3 product of such values reaches 1140 - 1230. The wave alternates between
 // the matrix cores (1024 cycles a tile) and the vector ALU (1000, half of it
 // exponentials); two workgroups a CU overlap them in part. Tried and not kept:
 // 64 rows a wave (half the LDS reads, one wave per SIMD: 675 us); 32-key steps
@@ -853,9 +854,9 @@ __device__ __forceinline__ void many_body(const PagedAttnArgs& a, uint16_t* lds,
 // Two column blocks of 128 dims take 346 registers where a CU holds one workgroup;
 // with two (256 registers) fewer LDS reads were in flight and 40 registers spilled.
 // us with two / with one: 16 requests of 4 tokens, 64 query and 8 kv heads, at up to
-// 2048 keys 35 / 30, 64 of them 97 / 82, 1 at 65535 67 / 59. (The other shapes are
-// not faster with one, and two blocks ahead in registers, 424 of them, took 32 / 88
-// / 62.)
+// 2048 keys 34.6 / 30.0, 64 of them 94 / 81, 1 at 65535 57.5 / 53.7. (The other shapes
+// are not faster with one, and two blocks ahead in registers, 424 of them, lost
+// another 2 - 6.)
 template <int HD, int NB>
 constexpr bool kWideFew = HD == 128 && NB == 2;
 
@@ -1085,21 +1086,24 @@ PagedAttnPlan paged_attn_plan(uint32_t n, uint32_t B, uint32_t hq, uint32_t hkv,
     p.many_sorted = B > 1 && B <= 64 && p.many_splits <= 2 && wgs * p.many_splits > 256;
   }
   // A workgroup a CU: four waves with a block each in flight draw what HBM gives.
-  // us at 128 / 256 / 512 / 1024 workgroups: 4 requests of up to 131071 keys 343 /
-  // 257 / 257 / 257, 16 of 4096 49 / 42 / 44 / 44, 64 of 2048 (70B heads) 70 / 70 /
-  // 70 / 78. At least kMinSplit keys each: 128, 256 and 512 are within 2 us, 1024
-  // loses 3 on 4 requests of 8192. Half of that beside longer requests, whose
-  // tiles fill the CUs too (12 x 511 rows and 36 single tokens of 64-wide heads at
-  // up to 2047 keys: 53 us with two splits and their joining, 49.6 without; a token
-  // each of 4 requests at 131071 and a chunk: 113, and 142 at 64 workgroups).
+  // us at 128 / 256 / 512 / 1024 workgroups, ragged lengths: 4 requests of up to 131071
+  // keys 332 / 235 / 198 / 196, 16 of 4096 41.5 / 34.6 / 34.6 / 33.4, 64 of 2048 (70B
+  // heads) 69.7 / 69.5 / 69.5 / 75.1, 4 of 8192 27.6 / 21.5 / 19.9 / 22.9; 16 x 4 rows
+  // of 70B heads at 2048 39 / 30 / 36 / 47, 1 x 4 at 65535 70 / 54 / 60 / 76. Half of
+  // that beside longer requests, whose tiles fill the CUs too; us at 128 / 256: 13
+  // single tokens beside 4 chunks of 155 rows at up to 1585 keys, 64-wide, 22.3 / 20.9,
+  // 36 beside 12 of 511 at 2047 50.1 / 48.6, 7 beside 14 of 351 at 1046 20.2 / 23.1,
+  // 35 beside 4 of 394 at 1234, 24:8 heads, 45.3 / 45.2 (a token each of 4 requests at
+  // 131071 and a chunk: 113, and 142 at 64 workgroups).
   // Not at all for one request, which the bound says has more rows (4096 rows of a
   // prompt behind 4095 keys: 5 us of joining nothing).
   const uint64_t wgs = std::max<uint64_t>(B * heads, 1), few_wgs = only_few ? 256 : B > 1 ? 128 : 1;
   p.few_splits = (uint32_t)std::min<uint64_t>((few_wgs + wgs - 1) / wgs, key_splits);
-  // Short contexts of few requests: eight waves and no second launch. us with it /
-  // with splits: one request of the 8B heads at 512 keys 9.4 / 11.8, at 1025 12.4 /
-  // 11.8, at 1536 15.1 / 11.6; 4 requests of 64-wide heads at 1025 8.9 / 11.6. (Two
-  // column blocks of 128 dims would spill: 21 us at 700 keys.)
+  // Short contexts of few requests: eight waves and no second launch. us a call with it
+  // / with splits (on the GPU alone): one request of the 8B heads at 512 keys 9.8 / 13.5
+  // (9.4 / 9.4), at 1025 13.6 / 13.5 (13.2 / 9.9), at 1536 16.9 / 13.6 (16.5 / 9.9); 4
+  // requests of 64-wide heads at 1025 10.0 / 13.7 (9.7 / 8.8). (Two column blocks of 128
+  // dims would spill: 21 us at 700 keys.)
   p.few_waves = 4;
   if (only_few && p.few_splits > 1 && (uint64_t)max_kv * hd <= 96 * 1024 && (p.few_blocks == 1 || hd == 64)) {
     p.few_waves = 8;
